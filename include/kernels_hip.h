@@ -220,6 +220,29 @@ int mynah_hip_q4k_int8_dev(const void *w, size_t rows, size_t cols, const int8_t
                            const float *xs, const int32_t *xsum, float *y, size_t tokens,
                            void *stream);
 
+/* Products in 8-bit floating point (e4m3: one sign, four exponent, three
+ * mantissa bits, no infinities, largest value 448) with an f32 scale for each
+ * 128 activations and each 128 x 128 block of the weights, as 8-bit checkpoints
+ * store them. No reference counterpart. Types are ggml's ids F32 = 0, F16 = 1,
+ * BF16 = 30; device pointers; asynchronous on `stream`; nothing is allocated.
+ * cols is a multiple of 16 (a last block may be shorter than 128); nb = ceil(cols
+ * / 128).
+ *
+ * x[tokens] of `type`, rows x_stride elements apart, to xq[tokens][cols] e4m3
+ * and xs[tokens][nb]: per block amax = max(max |x|, 2^-100), xs = amax *
+ * f32(1 / 448), xq = e4m3(x * (448 * (1 / amax))), each operation rounded to 32
+ * bits, e4m3 to nearest, ties to even. A NaN stays one; an infinity makes its
+ * block's scale infinite. x, its rows and xq 16-byte aligned. */
+int mynah_hip_fp8_quantize_dev(int type, const void *x, size_t x_stride, size_t tokens,
+                               size_t cols, uint8_t *xq, float *xs, void *stream);
+/* y[tokens][rows] of `type` from w[rows][cols] e4m3 with ws[ceil(rows / 128)][nb]:
+ * y[t][r] = sum over the blocks b of xs[t][b] ws[r / 128][b] sum_k xq[t][k]
+ * w[r][k], the sums in 32 bits, rounded to `type` once. Any tokens and rows
+ * from 1 on; w and xq 16-byte aligned. */
+int mynah_hip_fp8_matmat_dev(const uint8_t *w, const float *ws, size_t rows, size_t cols,
+                             const uint8_t *xq, const float *xs, int type, void *y,
+                             size_t tokens, void *stream);
+
 /* No counterpart in the reference. For callers that cannot allocate device
  * memory — code under HIP graph (stream) capture, serving loops that must
  * not allocate, harnesses that forbid hipMalloc: the int8 lane's product

@@ -14,3 +14,6 @@
 #include "sample.hip"
 #include "copy.hip"
 #include "int8.hip"
+#include "rope.hip"
+#include "fp8.hip"
+#include "tree_attn.hip"

@@ -118,7 +118,58 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_Q5K_GEMM_INT8_32_32, "mynah_q5k_gemm_int8_32x32") \
     X(MYNAH_K_Q5K_GEMM_INT8_64_64, "mynah_q5k_gemm_int8_64x64") \
     X(MYNAH_K_Q5K_GEMM_INT8_96_128, "mynah_q5k_gemm_int8_96x128") \
-    X(MYNAH_K_Q5K_GEMM_INT8_128_128, "mynah_q5k_gemm_int8_128x128")
+    X(MYNAH_K_Q5K_GEMM_INT8_128_128, "mynah_q5k_gemm_int8_128x128") \
+    X(MYNAH_K_ROPE, "mynah_rope_f32_f32") \
+    X(MYNAH_K_ROPE_F32_F16, "mynah_rope_f32_f16") \
+    X(MYNAH_K_ROPE_F32_BF16, "mynah_rope_f32_bf16") \
+    X(MYNAH_K_ROPE_F16_F32, "mynah_rope_f16_f32") \
+    X(MYNAH_K_ROPE_F16_F16, "mynah_rope_f16_f16") \
+    X(MYNAH_K_ROPE_F16_BF16, "mynah_rope_f16_bf16") \
+    X(MYNAH_K_ROPE_BF16_F32, "mynah_rope_bf16_f32") \
+    X(MYNAH_K_ROPE_BF16_F16, "mynah_rope_bf16_f16") \
+    X(MYNAH_K_ROPE_BF16_BF16, "mynah_rope_bf16_bf16") \
+    X(MYNAH_K_FP8_QUANT, "mynah_fp8_quantize_f32") \
+    X(MYNAH_K_FP8_QUANT_F16, "mynah_fp8_quantize_f16") \
+    X(MYNAH_K_FP8_QUANT_BF16, "mynah_fp8_quantize_bf16") \
+    X(MYNAH_K_FP8_FEW1, "mynah_fp8_few1_f32") \
+    X(MYNAH_K_FP8_FEW1_F16, "mynah_fp8_few1_f16") \
+    X(MYNAH_K_FP8_FEW1_BF16, "mynah_fp8_few1_bf16") \
+    X(MYNAH_K_FP8_FEW2, "mynah_fp8_few2_f32") \
+    X(MYNAH_K_FP8_FEW2_F16, "mynah_fp8_few2_f16") \
+    X(MYNAH_K_FP8_FEW2_BF16, "mynah_fp8_few2_bf16") \
+    X(MYNAH_K_FP8_FEW4, "mynah_fp8_few4_f32") \
+    X(MYNAH_K_FP8_FEW4_F16, "mynah_fp8_few4_f16") \
+    X(MYNAH_K_FP8_FEW4_BF16, "mynah_fp8_few4_bf16") \
+    X(MYNAH_K_TREE_F32, "mynah_tree_attn_f32_64_1") \
+    X(MYNAH_K_TREE_F32_64_2, "mynah_tree_attn_f32_64_2") \
+    X(MYNAH_K_TREE_F32_128_1, "mynah_tree_attn_f32_128_1") \
+    X(MYNAH_K_TREE_F32_128_2, "mynah_tree_attn_f32_128_2") \
+    X(MYNAH_K_TREE_F32_256_1, "mynah_tree_attn_f32_256_1") \
+    X(MYNAH_K_TREE_F16, "mynah_tree_attn_f16_64_1") \
+    X(MYNAH_K_TREE_F16_64_2, "mynah_tree_attn_f16_64_2") \
+    X(MYNAH_K_TREE_F16_64_4, "mynah_tree_attn_f16_64_4") \
+    X(MYNAH_K_TREE_F16_128_1, "mynah_tree_attn_f16_128_1") \
+    X(MYNAH_K_TREE_F16_128_2, "mynah_tree_attn_f16_128_2") \
+    X(MYNAH_K_TREE_F16_128_4, "mynah_tree_attn_f16_128_4") \
+    X(MYNAH_K_TREE_F16_256_1, "mynah_tree_attn_f16_256_1") \
+    X(MYNAH_K_TREE_F16_256_2, "mynah_tree_attn_f16_256_2") \
+    X(MYNAH_K_TREE_BF16, "mynah_tree_attn_bf16_64_1") \
+    X(MYNAH_K_TREE_BF16_64_2, "mynah_tree_attn_bf16_64_2") \
+    X(MYNAH_K_TREE_BF16_64_4, "mynah_tree_attn_bf16_64_4") \
+    X(MYNAH_K_TREE_BF16_128_1, "mynah_tree_attn_bf16_128_1") \
+    X(MYNAH_K_TREE_BF16_128_2, "mynah_tree_attn_bf16_128_2") \
+    X(MYNAH_K_TREE_BF16_128_4, "mynah_tree_attn_bf16_128_4") \
+    X(MYNAH_K_TREE_BF16_256_1, "mynah_tree_attn_bf16_256_1") \
+    X(MYNAH_K_TREE_BF16_256_2, "mynah_tree_attn_bf16_256_2") \
+    X(MYNAH_K_TREE_JOIN, "mynah_tree_join_f32_64") \
+    X(MYNAH_K_TREE_JOIN_F32_128, "mynah_tree_join_f32_128") \
+    X(MYNAH_K_TREE_JOIN_F32_256, "mynah_tree_join_f32_256") \
+    X(MYNAH_K_TREE_JOIN_F16_64, "mynah_tree_join_f16_64") \
+    X(MYNAH_K_TREE_JOIN_F16_128, "mynah_tree_join_f16_128") \
+    X(MYNAH_K_TREE_JOIN_F16_256, "mynah_tree_join_f16_256") \
+    X(MYNAH_K_TREE_JOIN_BF16_64, "mynah_tree_join_bf16_64") \
+    X(MYNAH_K_TREE_JOIN_BF16_128, "mynah_tree_join_bf16_128") \
+    X(MYNAH_K_TREE_JOIN_BF16_256, "mynah_tree_join_bf16_256")
 
 enum {
 #define X(id, name) id,
@@ -144,6 +195,8 @@ enum {
  * common.hip.h); the kernels for 2 and 4 query heads per key head take 32, 64 or
  * 128, chosen by the context length. */
 #define MYNAH_AS_CH 32
+/* Waves of a tree attention workgroup (= TA_WAVES in tree_attn.hip). */
+#define MYNAH_TA_WAVES 4u
 /* Most chunks mynah_attn_combine1 (one wave per query head) takes. */
 #define MYNAH_AC1_MAX 32
 
@@ -277,6 +330,36 @@ int mynah_gemv_group_geometry(mynah_gemv_group *grp, int order, uint32_t *thread
 int mynah_gemv_prefetch_plan(const mynah_gemv_group *next, int order, uint32_t wgs,
                              uint32_t bytes_per_wg, uint64_t max_bytes, uint32_t step_log2,
                              mynah_gemv_prefetch *pf);
+
+/* Host mirrors of rope.hip RopeSeg and RopeArgs. */
+typedef struct {
+    const void *in;
+    void *out;
+    size_t in_token, in_head, out_token, out_head;
+    const float *norm;
+    uint32_t heads, rotate, slotted, pad;
+} mynah_rope_seg;
+typedef struct {
+    mynah_rope_seg seg[3];
+    const double *freqs;
+    const int32_t *pos, *slots;
+    unsigned long long units;
+    uint32_t n_slots, hd, rot, lanes_log2, groups, heads;
+    float eps, mscale;
+} mynah_rope_args;
+/* Host mirror of tree_attn.hip TreeArgs. */
+typedef struct {
+    const void *q, *k, *v;
+    void *out;
+    size_t q_stride, out_stride, slot_stride, seq_slots;
+    const int32_t *pages, *seq_start, *n_past;
+    const uint32_t *mask;
+    float *pm, *pl, *po;
+    unsigned long long n_slots;
+    uint32_t n_seqs, n_heads, n_kv, group, n_rows, page_log2, max_pages, mask_words;
+    uint32_t max_nodes, max_kv, splits;
+    float scale2;
+} mynah_tree_args;
 
 /* Y[tokens][rows] = (res +) X[tokens][cols] · W^T in the matvec summation
  * order (every output bit-identical to the matvec of its token);

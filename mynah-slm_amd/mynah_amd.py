@@ -59,6 +59,39 @@ class GenTiming(C.Structure):
                 ("n_prompt", C.c_uint32), ("n_gen", C.c_uint32), ("ttft_done", C.c_int)]
 
 
+class RopeParams(C.Structure):
+    """mynah_rope_params (include/mynah_attention.h)."""
+    _fields_ = [("rot_dim", C.c_uint32), ("scaling", C.c_int), ("theta", C.c_double),
+                ("factor", C.c_double), ("trained", C.c_double), ("high", C.c_double),
+                ("low", C.c_double), ("mscale", C.c_double)]
+
+
+class QkNormRope(C.Structure):
+    """mynah_qk_norm_rope (include/mynah_attention.h); device addresses."""
+    _fields_ = [("type", C.c_int), ("out_type", C.c_int), ("layout", C.c_int),
+                ("n_heads", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("rot_dim", C.c_uint32), ("tokens", C.c_size_t), ("q", C.c_void_p),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_size_t),
+                ("k_stride", C.c_size_t), ("v_stride", C.c_size_t), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float), ("mscale", C.c_float),
+                ("freqs", C.c_void_p), ("pos", C.c_void_p), ("slots", C.c_void_p),
+                ("n_slots", C.c_size_t), ("q_out", C.c_void_p), ("q_out_stride", C.c_size_t),
+                ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("slot_stride", C.c_size_t)]
+
+
+class TreeAttention(C.Structure):
+    """mynah_tree_attention (include/mynah_attention.h); device addresses."""
+    _fields_ = [("type", C.c_int), ("n_seqs", C.c_uint32), ("n_heads", C.c_uint32),
+                ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("q", C.c_void_p),
+                ("q_stride", C.c_size_t), ("out", C.c_void_p), ("out_stride", C.c_size_t),
+                ("n_rows", C.c_uint32), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("slot_stride", C.c_size_t), ("n_slots", C.c_size_t), ("seq_slots", C.c_size_t),
+                ("pages", C.c_void_p), ("page_size", C.c_uint32), ("max_pages", C.c_uint32),
+                ("seq_start", C.c_void_p), ("n_past", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_words", C.c_uint32), ("max_nodes", C.c_uint32), ("max_kv", C.c_uint32),
+                ("scale", C.c_float)]
+
+
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint32)
 
 
@@ -87,6 +120,14 @@ def _load() -> C.CDLL:
         "mynah_hip_q4k_int8_dev": (C.c_int, [_P, _SZ, _SZ, _P, _P, _P, _P, _SZ, _P]),
         "mynah_hip_int8_product_noalloc_dev": (C.c_int, [C.c_int, _P, _SZ, _SZ, _P, _P, _SZ,
                                                          _P]),
+        "mynah_hip_fp8_quantize_dev": (C.c_int, [C.c_int, _P, _SZ, _SZ, _SZ, _P, _P, _P]),
+        "mynah_hip_fp8_matmat_dev": (C.c_int, [_P, _P, _SZ, _SZ, _P, _P, C.c_int, _P, _SZ, _P]),
+        "mynah_hip_rope_freqs": (C.c_int, [C.POINTER(RopeParams), _P, C.POINTER(C.c_float)]),
+        "mynah_hip_rope_dev": (C.c_int, [C.c_int, C.c_int, _P, _SZ, _SZ, _P, _SZ, _SZ, _SZ, _SZ,
+                                         C.c_uint32, C.c_uint32, _P, C.c_float, _P, _P]),
+        "mynah_hip_qk_norm_rope_dev": (C.c_int, [C.POINTER(QkNormRope), _P]),
+        "mynah_hip_tree_attention_workspace": (_SZ, [C.POINTER(TreeAttention)]),
+        "mynah_hip_tree_attention_dev": (C.c_int, [C.POINTER(TreeAttention), _P, _SZ, _P]),
         "mynah_hip_init": (C.c_int, [C.c_int]),
         "mynah_hip_last_error": (C.c_char_p, []),
         "mynah_hip_register": (C.c_int, [_P, _SZ]),
@@ -364,6 +405,59 @@ def matmat_dev(qtype: int, w: int, rows: int, cols: int, x: int, y: int, tokens:
 
 def dequant_dev(qtype: int, w: int, rows: int, cols: int, y: int, stream=None) -> None:
     check(lib.mynah_hip_dequant_dev(qtype, w, rows, cols, y, stream), "dequant_dev")
+
+
+# Element types of the operators below (ggml's ids).
+F32, F16, BF16 = 0, 1, 30
+
+
+def fp8_quantize_dev(qtype: int, x: int, x_stride: int, tokens: int, cols: int, xq: int, xs: int,
+                     stream=None) -> None:
+    check(lib.mynah_hip_fp8_quantize_dev(qtype, x, x_stride, tokens, cols, xq, xs, stream),
+          "fp8_quantize")
+
+
+def fp8_matmat_dev(w: int, ws: int, rows: int, cols: int, xq: int, xs: int, qtype: int, y: int,
+                   tokens: int, stream=None) -> None:
+    check(lib.mynah_hip_fp8_matmat_dev(w, ws, rows, cols, xq, xs, qtype, y, tokens, stream),
+          "fp8_matmat")
+
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_NONE, ROPE_LINEAR, ROPE_YARN, ROPE_BANDS = 0, 1, 2, 3
+
+
+def rope_freqs(rot_dim: int, theta: float, scaling: int = ROPE_NONE, factor: float = 1.0,
+               trained: float = 0.0, high: float = 0.0, low: float = 0.0, mscale: float = 0.0):
+    """(radians per position of each pair, the factor of cos and sin); no device needed."""
+    p = RopeParams(rot_dim, scaling, theta, factor, trained, high, low, mscale)
+    out, m = np.empty(max(rot_dim // 2, 1), np.float64), C.c_float(0.0)
+    check(lib.mynah_hip_rope_freqs(C.byref(p), ptr(out), C.byref(m)), "rope_freqs")
+    return out, float(m.value)
+
+
+def rope_dev(qtype: int, layout: int, x: int, x_token: int, x_head: int, y: int, y_token: int,
+             y_head: int, tokens: int, heads: int, head_dim: int, rot_dim: int, freqs: int,
+             mscale: float, pos: int, stream=None) -> None:
+    check(lib.mynah_hip_rope_dev(qtype, layout, x, x_token, x_head, y, y_token, y_head, tokens,
+                                 heads, head_dim, rot_dim, freqs, mscale, pos, stream), "rope")
+
+
+def qk_norm_rope_dev(args: QkNormRope, stream=None) -> None:
+    check(lib.mynah_hip_qk_norm_rope_dev(args, stream), "qk_norm_rope")
+
+
+def tree_attention_workspace(args: TreeAttention) -> int:
+    n = int(lib.mynah_hip_tree_attention_workspace(args))
+    if n == 0:
+        raise HipError(f"tree_attention: {lib.mynah_hip_last_error().decode(errors='replace')}")
+    return n
+
+
+def tree_attention_dev(args: TreeAttention, workspace: int, workspace_bytes: int,
+                       stream=None) -> None:
+    check(lib.mynah_hip_tree_attention_dev(args, workspace, workspace_bytes, stream),
+          "tree_attention")
 
 
 def copy_dev(dst: int, src: int, nbytes: int, stream=None) -> None:
