@@ -6,6 +6,8 @@
 #include "mynah_attention.h"
 #include "runtime_internal.h"
 
+#include <stdlib.h>
+
 #define BLOCK 128u
 
 static int type_index(int type) {
@@ -56,6 +58,52 @@ int mynah_hip_fp8_quantize_dev(int type, const void *x, size_t x_stride, size_t 
                         256, 0, mynah_stream_or_default(d, stream), args);
 }
 
+/* The tiled kernels, in the kernel ids' order (the largest has no f32 form): how
+ * many workgroups a CU holds, and the microseconds of a step (a block of 128
+ * columns) with one a CU and with all of them, for 16-bit and for f32 outputs,
+ * measured on MI355X as the slope from 10 to 40 blocks at 256 workgroups and at
+ * 2,048. Two of the 4-wave 128 x 128 tile share a CU (1.17 us for both); alone on
+ * it the 8-wave one is the faster (0.65 against 0.78). */
+typedef struct {
+    uint32_t rows, toks, waves, per_cu;
+    float one[2], all[2];
+} fp8_tile;
+static const fp8_tile fp8_tiles[5] = {
+    {64, 64, 4, 2, {0.29f, 0.42f}, {0.45f, 0.67f}},
+    {64, 128, 4, 2, {0.48f, 0.67f}, {0.82f, 1.15f}},
+    {128, 128, 4, 2, {0.78f, 1.06f}, {1.17f, 1.85f}},
+    {128, 128, 8, 1, {0.65f, 1.09f}, {0.65f, 1.10f}},
+    {256, 256, 8, 1, {1.82f, 0.0f}, {2.00f, 0.0f}}};
+
+/* The tile of least estimated time for a product, or NULL for the streaming
+ * kernel: whole rounds of resident workgroups, then a last one. Four steps stand
+ * for the start and the end of a workgroup. The tiles address their rows in 32
+ * bits. MYNAH_FP8_TILE=0..4 forces one. */
+static const fp8_tile *fp8_plan(int type, size_t rows, size_t tokens, size_t cols,
+                                uint32_t cus) {
+    const int f32 = type == MYNAH_F32, most = f32 ? 3 : 4;
+    if (tokens <= 64 || cols > (size_t)1 << 23) return NULL;
+    const char *env = getenv("MYNAH_FP8_TILE");
+    if (env != NULL && env[0] >= '0' && env[0] <= '0' + most && env[1] == '\0')
+        return &fp8_tiles[env[0] - '0'];
+    const fp8_tile *best = NULL;
+    double best_us = 0.0;
+    for (int i = 0; i <= most; i++) {
+        const fp8_tile *t = &fp8_tiles[i];
+        const uint64_t wgs = (uint64_t)((rows + t->rows - 1) / t->rows) *
+                             (uint64_t)((tokens + t->toks - 1) / t->toks);
+        const uint64_t slots = (uint64_t)cus * t->per_cu, left = wgs % slots;
+        double us = (double)(wgs / slots) * t->all[f32];
+        if (left) us += left <= cus ? t->one[f32] : t->all[f32];
+        us *= (double)((cols + BLOCK - 1) / BLOCK + 4);
+        if (best == NULL || us < best_us) {
+            best = t;
+            best_us = us;
+        }
+    }
+    return best;
+}
+
 int mynah_hip_fp8_matmat_dev(const uint8_t *w, const float *ws, size_t rows, size_t cols,
                              const uint8_t *xq, const float *xs, int type, void *y,
                              size_t tokens, void *stream) {
@@ -79,6 +127,18 @@ int mynah_hip_fp8_matmat_dev(const uint8_t *w, const float *ws, size_t rows, siz
     uint32_t r32 = (uint32_t)rows, c32 = (uint32_t)cols, t32 = (uint32_t)tokens,
              nb = (uint32_t)((cols + BLOCK - 1) / BLOCK);
     hipStream_t st = mynah_stream_or_default(d, stream);
+    const int t = type_index(type);
+    const fp8_tile *tl = fp8_plan(type, rows, tokens, cols, (uint32_t)d->cus);
+    if (tl != NULL) {
+        uint32_t tr = (uint32_t)((rows + tl->rows - 1) / tl->rows);
+        const uint64_t wgs = (uint64_t)tr * ((tokens + tl->toks - 1) / tl->toks);
+        if (wgs <= 0x7fffffffu) {
+            void *args[] = {&w, &ws, &xq, &xs, &y, &r32, &c32, &t32, &nb, &tr};
+            return mynah_launch(d, MYNAH_K_FP8_TILE + 3 * (int)(tl - fp8_tiles) + t -
+                                (tl == &fp8_tiles[4]), (unsigned)wgs,
+                                1, 64 * tl->waves, 0, st, args);
+        }
+    }
     void *args[] = {&w, &ws, &xq, &xs, &y, &r32, &c32, &t32, &nb};
     const int v = tokens <= 16 ? 0 : tokens <= 32 ? 1 : 2;
     const uint32_t per = 16u << v;
@@ -87,6 +147,6 @@ int mynah_hip_fp8_matmat_dev(const uint8_t *w, const float *ws, size_t rows, siz
         mynah_set_error("fp8: too many tokens for one launch");
         return -1;
     }
-    return mynah_launch(d, MYNAH_K_FP8_FEW1 + 3 * v + type_index(type),
-                        (unsigned)((rows + 15) / 16), (unsigned)tiles, 256, 0, st, args);
+    return mynah_launch(d, MYNAH_K_FP8_FEW1 + 3 * v + t, (unsigned)((rows + 15) / 16),
+                        (unsigned)tiles, 256, 0, st, args);
 }
