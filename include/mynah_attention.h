@@ -119,8 +119,8 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  * node i sees node j where bit j % 32 of mask[row of i][j / 32] is set.
  *   out[row][h] = sum_p softmax_p(scale q[row][h] . k[p][h / group]) v[p][h / group]
  * over the seen positions p, group = n_heads / n_kv_heads; a row that sees
- * nothing, or scores of -inf only, is 0. Unseen positions have no effect, whatever their keys and
- * values hold. mask NULL: node i sees nodes 0 .. i (a chain: several tokens
+ * nothing, or scores of -inf only, is 0. Unseen positions have no effect,
+ * whatever their keys and values hold. mask NULL: node i sees nodes 0 .. i (a chain: several tokens
  * in order, or one). Statistics and sums are held in 32 bits; of 16-bit types
  * the probabilities are rounded to the type for the product with V, the
  * result once. The sums' order depends on the sizes and max_* values alone, so
@@ -136,7 +136,7 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  *     touched, and a negative n_past counts as 0;
  *   - head_dim 64, 128 or 256; 1 <= n_heads / n_kv_heads <= 64; page_size a
  *     power of two from 16 on; q, out, caches and strides aligned to 16 bytes;
- *     max_kv <= 2^26, and with a mask max_nodes <= 32 * mask_words. */
+ *     slot_stride below 2^24 bytes; max_kv <= 2^26, and with a mask max_nodes <= 32 * mask_words. */
 typedef struct {
     int type;                                   /* of q, out and the caches */
     uint32_t n_seqs, n_heads, n_kv_heads, head_dim;

@@ -8,6 +8,7 @@
 #include "runtime_internal.h"
 
 #include <math.h>
+#include <stdlib.h>
 #include <string.h>
 
 #define PI 3.14159265358979323846
@@ -220,14 +221,11 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *p, void *stream) {
 
 /* ── attention of drafted tokens over a cache ────────────────────────────── */
 
-/* Workgroups that keep the chip's loads in flight: four a CU. */
-#define TREE_WGS_PER_CU 4u
-#define TREE_MAX_SPLITS 256u
-
-/* What a call launches: 16 * nt query rows a workgroup, positions in `splits`
+/* What a call launches: kernel `variant` of its type and head size, 16 * nt query
+ * rows for each of rw row waves, `waves` waves a workgroup, positions in `splits`
  * runs. */
 typedef struct {
-    uint32_t nt, groups, splits;
+    uint32_t variant, nt, rw, waves, groups, splits;
 } tree_plan;
 
 static int tree_check(const mynah_tree_attention *p) {
@@ -263,7 +261,7 @@ static int tree_check(const mynah_tree_attention *p) {
     }
     const size_t qh = p->n_heads * hd, kh = p->n_kv_heads * hd;
     if (p->q_stride < qh || p->out_stride < qh || p->slot_stride < kh ||
-        p->slot_stride > (size_t)1 << 24 || !fits(p->n_rows, p->q_stride, qh, size) ||
+        p->slot_stride >= ((size_t)1 << 24) / size || !fits(p->n_rows, p->q_stride, qh, size) ||
         !fits(p->n_rows, p->out_stride, qh, size))
         return refuse("tree_attention: bad stride");
     if ((((uintptr_t)p->q | (uintptr_t)p->out | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache) &
@@ -279,19 +277,37 @@ static int tree_check(const mynah_tree_attention *p) {
 static void tree_make_plan(const mynah_tree_attention *p, uint32_t cus, tree_plan *t) {
     const uint32_t group = p->n_heads / p->n_kv_heads;
     const uint64_t tiles = ((uint64_t)p->max_nodes * group + 15) / 16;
-    /* Column tiles that fit the registers beside a chunk of keys and values. */
-    const uint32_t most = p->type == MYNAH_F32 ? (p->head_dim == 256 ? 1u : 2u)
-                                               : (p->head_dim == 256 ? 2u : 4u);
-    t->nt = tiles >= 3 ? 4u : (uint32_t)tiles;
-    if (t->nt > most) t->nt = most;
-    t->groups = (uint32_t)((tiles + t->nt - 1) / t->nt);
+    const int f32 = p->type == MYNAH_F32, wide = p->head_dim == 256;
+    t->waves = wide ? 4u : 8u;
+    t->nt = 1;
+    if (f32) {
+        /* More row waves leave a workgroup fewer keys at a time and more of them
+         * idle at the ends: 96 rows over 2072 positions, 22 us with two, 30 with
+         * four, 35 with eight. */
+        t->variant = tiles > 1 ? 1u : 0u;
+        t->rw = t->variant + 1u;
+    } else if (wide) {
+        t->variant = tiles > 2 ? 2u : (uint32_t)tiles - 1u;
+        t->rw = 1u << t->variant;
+    } else {
+        /* Every row of the call in one workgroup as far as that goes, for its keys
+         * then come from memory once: 256 rows over 130,001 positions, 202 us with
+         * 2 x 8 tiles, 278 with every wave on keys of its own. */
+        t->variant = tiles > 8 ? 4u : tiles > 4 ? 3u : tiles > 2 ? 2u : (uint32_t)tiles - 1u;
+        if (t->variant == 4u && p->head_dim == 64) t->variant = 3u;
+        t->nt = t->variant > 1u ? 2u : 1u;
+        t->rw = t->variant == 0u ? 1u : 1u << (t->variant - (t->nt == 2u));
+    }
+    t->groups = (uint32_t)((tiles + t->nt * t->rw - 1) / (t->nt * t->rw));
+    /* One workgroup fills a CU's LDS, so at most one for each CU: 264 on 256 CUs
+     * took 39 us where 240 take 22. Two or three turns of smaller ones are slower
+     * too (16 sequences of 8192 bf16 positions 99, 109 and 121 us). */
     const uint64_t base = (uint64_t)p->n_seqs * p->n_kv_heads * t->groups;
-    const uint32_t step = MYNAH_TA_WAVES * (p->type == MYNAH_F32 ? 16u : 32u);
-    uint64_t s = ((uint64_t)cus * TREE_WGS_PER_CU + base - 1) / base;
-    const uint64_t chunks = (p->max_kv + step - 1) / step;
-    if (s > chunks) s = chunks;
-    if (s > TREE_MAX_SPLITS) s = TREE_MAX_SPLITS;
-    t->splits = (uint32_t)s;
+    const uint32_t turn = t->waves / t->rw * (f32 ? 16u : 32u) * (t->rw > 1 ? 2u : 1u);
+    const uint64_t turns = (p->max_kv + turn - 1) / turn;
+    uint64_t s = cus / base;
+    if (s > turns) s = turns;
+    t->splits = s ? (uint32_t)s : 1u;
 }
 
 static size_t tree_ws(const mynah_tree_attention *p, const tree_plan *t) {
@@ -308,11 +324,13 @@ size_t mynah_hip_tree_attention_workspace(const mynah_tree_attention *p) {
     return tree_ws(p, &t);
 }
 
-static int tree_kernel(const mynah_tree_attention *p, uint32_t nt) {
-    const int h = p->head_dim == 64 ? 0 : p->head_dim == 128 ? 1 : 2;
-    const int n = nt == 1 ? 0 : nt == 2 ? 1 : 2;
-    if (p->type == MYNAH_F32) return MYNAH_K_TREE_F32 + 2 * h + n;
-    return MYNAH_K_TREE_F16 + 8 * (p->type == MYNAH_BF16) + 3 * h + n;
+static int tree_kernel(const mynah_tree_attention *p, uint32_t variant) {
+    /* The first variant of head sizes 64, 128 and 256, in the kernel ids' order. */
+    static const int first[2][3] = {{0, 4, 9}, {0, 2, 4}};
+    const int h = p->head_dim == 64 ? 0 : p->head_dim == 128 ? 1 : 2, f32 = p->type == MYNAH_F32;
+    const int type = f32 ? MYNAH_K_TREE_F32
+                         : p->type == MYNAH_F16 ? MYNAH_K_TREE_F16 : MYNAH_K_TREE_BF16;
+    return type + first[f32][h] + (int)variant;
 }
 
 int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
@@ -360,11 +378,18 @@ int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
     a.max_nodes = p->max_nodes;
     a.max_kv = p->max_kv;
     a.splits = t.splits;
-    a.scale2 = p->scale * 1.44269504088896341f;
+    a.groups = t.groups;
+    /* Queries change sign where the scale is negative; no scale counts as a
+     * very small one (a score of 0 within 2^-20 for products up to 10^24), so
+     * that -inf stays what it is. */
+    a.scale2 = fabsf(p->scale) * 1.44269504088896341f;
+    if (a.scale2 < 1e-30f) a.scale2 = 1e-30f;
+    if (p->scale < 0.0f) a.flip = p->type == MYNAH_F32 ? 0x80000000u : 0x80008000u;
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a};
-    if (mynah_launch3(d, tree_kernel(p, t.nt), p->n_seqs * p->n_kv_heads, t.splits, t.groups,
-                      64 * MYNAH_TA_WAVES, 0, st, args) != 0)
+    const uint64_t wgs = (uint64_t)p->n_seqs * t.splits * p->n_kv_heads * t.groups;
+    if (wgs > 0x7fffffffu) return refuse("tree_attention: too many workgroups for one launch");
+    if (mynah_launch(d, tree_kernel(p, t.variant), (unsigned)wgs, 1, 64 * t.waves, 0, st, args) != 0)
         return -1;
     if (t.splits < 2) return 0;
     const int h = p->head_dim == 64 ? 0 : p->head_dim == 128 ? 1 : 2;

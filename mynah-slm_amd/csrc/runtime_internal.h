@@ -154,27 +154,36 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_FP8_128X128W_BF16, "mynah_fp8_128x128w_bf16") \
     X(MYNAH_K_FP8_256X256_F16, "mynah_fp8_256x256_f16") \
     X(MYNAH_K_FP8_256X256_BF16, "mynah_fp8_256x256_bf16") \
-    X(MYNAH_K_TREE_F32, "mynah_tree_attn_f32_64_1") \
-    X(MYNAH_K_TREE_F32_64_2, "mynah_tree_attn_f32_64_2") \
-    X(MYNAH_K_TREE_F32_128_1, "mynah_tree_attn_f32_128_1") \
-    X(MYNAH_K_TREE_F32_128_2, "mynah_tree_attn_f32_128_2") \
-    X(MYNAH_K_TREE_F32_256_1, "mynah_tree_attn_f32_256_1") \
-    X(MYNAH_K_TREE_F16, "mynah_tree_attn_f16_64_1") \
-    X(MYNAH_K_TREE_F16_64_2, "mynah_tree_attn_f16_64_2") \
-    X(MYNAH_K_TREE_F16_64_4, "mynah_tree_attn_f16_64_4") \
-    X(MYNAH_K_TREE_F16_128_1, "mynah_tree_attn_f16_128_1") \
-    X(MYNAH_K_TREE_F16_128_2, "mynah_tree_attn_f16_128_2") \
-    X(MYNAH_K_TREE_F16_128_4, "mynah_tree_attn_f16_128_4") \
-    X(MYNAH_K_TREE_F16_256_1, "mynah_tree_attn_f16_256_1") \
-    X(MYNAH_K_TREE_F16_256_2, "mynah_tree_attn_f16_256_2") \
-    X(MYNAH_K_TREE_BF16, "mynah_tree_attn_bf16_64_1") \
-    X(MYNAH_K_TREE_BF16_64_2, "mynah_tree_attn_bf16_64_2") \
-    X(MYNAH_K_TREE_BF16_64_4, "mynah_tree_attn_bf16_64_4") \
-    X(MYNAH_K_TREE_BF16_128_1, "mynah_tree_attn_bf16_128_1") \
-    X(MYNAH_K_TREE_BF16_128_2, "mynah_tree_attn_bf16_128_2") \
-    X(MYNAH_K_TREE_BF16_128_4, "mynah_tree_attn_bf16_128_4") \
-    X(MYNAH_K_TREE_BF16_256_1, "mynah_tree_attn_bf16_256_1") \
-    X(MYNAH_K_TREE_BF16_256_2, "mynah_tree_attn_bf16_256_2") \
+    X(MYNAH_K_TREE_F32, "mynah_tree_attn_f32_64_1x1") \
+    X(MYNAH_K_TREE_F32_64_1X2, "mynah_tree_attn_f32_64_1x2") \
+    X(MYNAH_K_TREE_F32_128_1X1, "mynah_tree_attn_f32_128_1x1") \
+    X(MYNAH_K_TREE_F32_128_1X2, "mynah_tree_attn_f32_128_1x2") \
+    X(MYNAH_K_TREE_F32_256_1X1, "mynah_tree_attn_f32_256_1x1") \
+    X(MYNAH_K_TREE_F32_256_1X2, "mynah_tree_attn_f32_256_1x2") \
+    X(MYNAH_K_TREE_F16, "mynah_tree_attn_f16_64_1x1") \
+    X(MYNAH_K_TREE_F16_64_1X2, "mynah_tree_attn_f16_64_1x2") \
+    X(MYNAH_K_TREE_F16_64_2X2, "mynah_tree_attn_f16_64_2x2") \
+    X(MYNAH_K_TREE_F16_64_2X4, "mynah_tree_attn_f16_64_2x4") \
+    X(MYNAH_K_TREE_F16_128_1X1, "mynah_tree_attn_f16_128_1x1") \
+    X(MYNAH_K_TREE_F16_128_1X2, "mynah_tree_attn_f16_128_1x2") \
+    X(MYNAH_K_TREE_F16_128_2X2, "mynah_tree_attn_f16_128_2x2") \
+    X(MYNAH_K_TREE_F16_128_2X4, "mynah_tree_attn_f16_128_2x4") \
+    X(MYNAH_K_TREE_F16_128_2X8, "mynah_tree_attn_f16_128_2x8") \
+    X(MYNAH_K_TREE_F16_256_1X1, "mynah_tree_attn_f16_256_1x1") \
+    X(MYNAH_K_TREE_F16_256_1X2, "mynah_tree_attn_f16_256_1x2") \
+    X(MYNAH_K_TREE_F16_256_1X4, "mynah_tree_attn_f16_256_1x4") \
+    X(MYNAH_K_TREE_BF16, "mynah_tree_attn_bf16_64_1x1") \
+    X(MYNAH_K_TREE_BF16_64_1X2, "mynah_tree_attn_bf16_64_1x2") \
+    X(MYNAH_K_TREE_BF16_64_2X2, "mynah_tree_attn_bf16_64_2x2") \
+    X(MYNAH_K_TREE_BF16_64_2X4, "mynah_tree_attn_bf16_64_2x4") \
+    X(MYNAH_K_TREE_BF16_128_1X1, "mynah_tree_attn_bf16_128_1x1") \
+    X(MYNAH_K_TREE_BF16_128_1X2, "mynah_tree_attn_bf16_128_1x2") \
+    X(MYNAH_K_TREE_BF16_128_2X2, "mynah_tree_attn_bf16_128_2x2") \
+    X(MYNAH_K_TREE_BF16_128_2X4, "mynah_tree_attn_bf16_128_2x4") \
+    X(MYNAH_K_TREE_BF16_128_2X8, "mynah_tree_attn_bf16_128_2x8") \
+    X(MYNAH_K_TREE_BF16_256_1X1, "mynah_tree_attn_bf16_256_1x1") \
+    X(MYNAH_K_TREE_BF16_256_1X2, "mynah_tree_attn_bf16_256_1x2") \
+    X(MYNAH_K_TREE_BF16_256_1X4, "mynah_tree_attn_bf16_256_1x4") \
     X(MYNAH_K_TREE_JOIN, "mynah_tree_join_f32_64") \
     X(MYNAH_K_TREE_JOIN_F32_128, "mynah_tree_join_f32_128") \
     X(MYNAH_K_TREE_JOIN_F32_256, "mynah_tree_join_f32_256") \
@@ -209,8 +218,6 @@ enum {
  * common.hip.h); the kernels for 2 and 4 query heads per key head take 32, 64 or
  * 128, chosen by the context length. */
 #define MYNAH_AS_CH 32
-/* Waves of a tree attention workgroup (= TA_WAVES in tree_attn.hip). */
-#define MYNAH_TA_WAVES 4u
 /* Most chunks mynah_attn_combine1 (one wave per query head) takes. */
 #define MYNAH_AC1_MAX 32
 
@@ -371,8 +378,9 @@ typedef struct {
     float *pm, *pl, *po;
     unsigned long long n_slots;
     uint32_t n_seqs, n_heads, n_kv, group, n_rows, page_log2, max_pages, mask_words;
-    uint32_t max_nodes, max_kv, splits;
+    uint32_t max_nodes, max_kv, splits, groups;
     float scale2;
+    uint32_t flip;
 } mynah_tree_args;
 
 /* Y[tokens][rows] = (res +) X[tokens][cols] · W^T in the matvec summation

@@ -6,20 +6,26 @@
 // Q^T, so that a lane holds four keys' scores of one query, which is what the
 // second product O^T = V^T P^T takes as its operand: the probabilities never
 // leave their registers. Which key and which dimension an operand's place
-// stands for is free as long as both operands agree, so K and V are read from
-// memory in whole runs of 8 or 16 bytes a lane into the operands' registers;
-// 16-bit V is turned by one v_perm per two values. No LDS in the loop and no
-// barrier: each wave walks its own chunks of keys with its own running maximum
-// and sum; the waves meet once at the end, workgroups in a second launch.
+// stands for is free as long as both operands agree, so K and V leave the LDS in
+// whole runs of 8 or 16 bytes a lane; 16-bit V is turned by one v_perm per two
+// values. The copies from memory go straight to the LDS (keys read from memory as
+// operands, 16 rows an instruction, came at 22-31 bytes a clock and CU, the rate of
+// the address unit) and stay under way while the chunk before is computed. Each
+// wave keeps a running maximum and sum for its own keys; the waves meet once at the
+// end, workgroups in a second launch.
+//
+// Bound by memory where a key head has few rows, by the matrix and exponential
+// units where it has many. Measured, MI355X: 16 sequences of 16 nodes over up to
+// 8207 bf16 positions in pages (32 heads, 8 of keys, 128 wide; 288 MB) 99 us, 2.9
+// TB/s; the same with one node each 78 us, 3.7 TB/s; 64 nodes over 130,065 f16
+// positions (533 MB, 136 GFLOP) 198 us; one sequence of 16 nodes over 65,552 60 us,
+// 4.5 TB/s, of one node 51 us, 5.2 TB/s; 24 f32 nodes over 2072 positions 21 us; one
+// f32 token over 513 13 us.
 //
 // SPDX-License-Identifier: MIT
 #pragma once
 #include "common.hip.h"
 #include "elem.hip.h"
-
-// Waves of a workgroup, each with its own keys (= MYNAH_TA_WAVES in
-// runtime_internal.h).
-#define TA_WAVES 4
 
 struct TreeArgs {
     const void *q, *k, *v;
@@ -30,13 +36,21 @@ struct TreeArgs {
     float *pm, *pl, *po;            // partials [split][n_rows * n_heads], (x head_dim)
     unsigned long long n_slots;
     uint32_t n_seqs, n_heads, n_kv, group, n_rows, page_log2, max_pages, mask_words;
-    uint32_t max_nodes, max_kv, splits;
-    float scale2;                   // scale * log2(e)
+    uint32_t max_nodes, max_kv, splits, groups;
+    float scale2;                   // |scale| log2(e), above 0
+    uint32_t flip;                  // sign bits of a query's dwords, where scale is below 0
 };
 
 typedef float ta_v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 ta_v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 ta_v8b __attribute__((ext_vector_type(8)));
+
+// A word that no kernel writes while this one runs, by a scalar load (of a plain
+// pointer the compiler takes a vector load, and its wait drains the prefetches).
+typedef __attribute__((address_space(4))) const int32_t ta_const_i32;
+MYNAH_DEV int32_t scalar_i32(const int32_t *p, size_t i) {
+    return ((ta_const_i32 *)(uintptr_t)p)[i];
+}
 
 struct SeqSpan {
     long long row0;                 // first query row
@@ -46,9 +60,9 @@ struct SeqSpan {
 // A sequence's rows and positions as the call bounds them.
 MYNAH_DEV SeqSpan seq_span(const TreeArgs &a, uint32_t b) {
     SeqSpan s;
-    s.row0 = a.seq_start[b];
-    const long long n = (long long)a.seq_start[b + 1u] - s.row0;
-    const int past = a.n_past[b];
+    s.row0 = scalar_i32(a.seq_start, b);
+    const long long n = (long long)scalar_i32(a.seq_start, b + 1u) - s.row0;
+    const int past = scalar_i32(a.n_past, b);
     s.nodes = n <= 0 ? 0u : n < (long long)a.max_nodes ? (uint32_t)n : a.max_nodes;
     s.past = past > 0 ? (uint32_t)past : 0u;
     const unsigned long long kv = (unsigned long long)s.past + s.nodes;
@@ -69,7 +83,15 @@ struct TaShape {
     static constexpr int CW = F32 || HD == 64 ? 4 : 8; // of them side by side
     static constexpr int VP = VE / CW;                // pieces of a lane's value row
     static constexpr int VD = CW * (int)sizeof(T) / 4; // dwords of a piece
+    static constexpr int KB = CK * HD * (int)sizeof(T); // bytes of a chunk's keys
+    static constexpr int CPR = HD * (int)sizeof(T) / 16; // 16-byte pieces of a key
+    static constexpr int RPI = 64 / CPR;              // keys that one copy takes
+    // Waves of a workgroup (= tree_plan.waves in attention.c): their chunks of keys
+    // and values, in flight or in use, fill the LDS.
+    static constexpr int W = HD == 256 ? 4 : 8;
 };
+
+typedef __attribute__((address_space(3))) void ta_lds_void;
 
 template <class T>
 MYNAH_DEV ta_v4f ta_mfma(const uint32_t (&a)[4], const uint32_t (&b)[4], ta_v4f c) {
@@ -106,29 +128,30 @@ MYNAH_DEV void load_dwords(const char *p, uint32_t *d) {
     }
 }
 
-// A register of one f32 or two 16-bit values: whether it holds an infinity or
-// NaN, and the register with zeros in their place.
+// A register of one f32 or two 16-bit values with zeros in the place of
+// infinities and NaN.
 template <class T>
 MYNAH_DEV uint32_t finite_part(uint32_t d) {
     if constexpr (sizeof(T) == 4) return (d & 0x7f800000u) == 0x7f800000u ? 0u : d;
     constexpr uint32_t e = __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
     return ((d & e) == e ? 0u : d & 0xffffu) | (((d >> 16) & e) == e ? 0u : d & 0xffff0000u);
 }
-template <class T>
-MYNAH_DEV bool not_finite(uint32_t d) { return finite_part<T>(d) != d; }
 
 // Whether a query (node `node` of its sequence, its words of the mask from
 // `words` on) sees node j, as 0 or 1.
 MYNAH_DEV uint32_t sees_node(const TreeArgs &a, size_t words, uint32_t node, uint32_t j) {
-    if (a.mask == nullptr) return j <= node;
-    return (a.mask[words + j / 32u] >> (j & 31u)) & 1u;
+    // Without a branch: a word that is there is read in any case.
+    const bool chain = a.mask == nullptr;
+    const uint32_t *p = chain ? (const uint32_t *)a.n_past : a.mask + words + j / 32u;
+    const uint32_t bit = (*p >> (j & 31u)) & 1u;
+    return chain ? (uint32_t)(j <= node) : bit;
 }
 
 // The cache row of position p of sequence b; false where it is not in the cache.
 MYNAH_DEV bool cache_row(const TreeArgs &a, uint32_t b, uint32_t p, unsigned long long &row) {
     unsigned long long r = (unsigned long long)b * a.seq_slots + p;
     if (a.pages) {
-        const int pg = a.pages[(size_t)b * a.max_pages + (p >> a.page_log2)];
+        const int pg = scalar_i32(a.pages, (size_t)b * a.max_pages + (p >> a.page_log2));
         if (pg < 0) return false;
         r = ((unsigned long long)(uint32_t)pg << a.page_log2) + (p & ((1u << a.page_log2) - 1u));
     }
@@ -136,30 +159,61 @@ MYNAH_DEV bool cache_row(const TreeArgs &a, uint32_t b, uint32_t p, unsigned lon
     return r < a.n_slots;
 }
 
-// Grid (n_seqs * n_kv, splits, row groups of 16 NT), block 64 TA_WAVES.
-template <class T, int HD, int NT>
+// Growth of a column's scores, in powers of two, that its reference for the
+// exponentials is left behind by: sums and 16-bit probabilities hold 2^8 times
+// their size, and most chunks then rescale nothing and compare only within
+// their lanes.
+#define TA_LAG 8.0f
+
+// A workgroup's W waves are RW row waves, each with 16 NT query rows of its own, for
+// each of W / RW key groups, which take chunks of keys in turn.
+//   RW == 1: a wave's chunk is its own, one buffer of keys and one of values: the
+//     next keys are copied when these are used up, values likewise; no barrier.
+//   RW > 1: the row waves of a key group copy its chunk together, two buffers, one
+//     barrier a chunk: what comes from the L2 is read by RW waves. (Alone, each wave
+//     with its own rows and keys, 256 rows over 130,001 f16 positions read 4.3 GB
+//     through the L2 at 14-16 TB/s, 278 us.)
+// Grid n_seqs * splits * n_kv * groups (of 16 NT RW query rows), block 64 W.
+// Workgroups go to the 8 XCDs in turn; each XCD takes a run of the order (sequence,
+// split, key head, group), so that groups that share keys share its L2.
+template <class T, int HD, int NT, int RW>
 MYNAH_DEV void tree_attn(const TreeArgs &a) {
     using S = TaShape<T, HD>;
-    __shared__ __attribute__((aligned(16))) float lo[TA_WAVES][16][HD + 4];
-    __shared__ float lm_[TA_WAVES][16], ll_[TA_WAVES][16];
-    __shared__ uint32_t lbad[TA_WAVES];
+    constexpr int KW = S::W / RW;                  // key groups
+    constexpr int BUF = KW * S::KB, HALF = S::W * S::KB / 2;
+    // A buffer of keys and one of values, or two of each: objects of their own, so
+    // that reads of one wait for its copies alone. Half of the waves' results (of the
+    // dimensions) takes the first one's place at the end.
+    __shared__ __attribute__((aligned(16))) uint8_t kx[BUF > HALF ? BUF : HALF], vx[BUF];
+    __shared__ __attribute__((aligned(16))) uint8_t ky[RW > 1 ? BUF : 16], vy[RW > 1 ? BUF : 16];
+    __shared__ float lmax[S::W][16], lsum[S::W][16];
+    __shared__ uint32_t lbad[S::W];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lane = threadIdx.x & 63u, lm = lane & 15u, lk = lane >> 4;
-    const uint32_t b = blockIdx.x / a.n_kv, kvh = blockIdx.x - b * a.n_kv, split = blockIdx.y;
+    const uint32_t rw = wave % RW, kg = wave / RW;
+    uint32_t id = blockIdx.x;
+    const uint32_t even = gridDim.x & ~7u;
+    if (id < even) id = (id & 7u) * (even >> 3) + (id >> 3);
+    const uint32_t head_id = id / a.groups, part = head_id / a.n_kv, b = part / a.splits;
+    const uint32_t kvh = head_id - part * a.n_kv, split = part - b * a.splits;
     const SeqSpan sq = seq_span(a, b);
-    const uint32_t rows = sq.nodes * a.group, rr0 = blockIdx.z * (16u * NT);
-    if (rr0 >= rows) return;                       // uniform
+    const uint32_t rows = sq.nodes * a.group;
+    const uint32_t wg0 = (id - head_id * a.groups) * (16u * NT * RW);
+    if (wg0 >= rows) return;                       // uniform
+    const uint32_t rr0 = wg0 + 16u * NT * rw;      // the wave's first row
+    const uint32_t turn = S::CK * KW;              // keys that the groups take at a time
     uint32_t per = (sq.kv + a.splits - 1u) / a.splits;
-    per = (per + S::CK * TA_WAVES - 1u) / (S::CK * TA_WAVES) * (S::CK * TA_WAVES);
+    per = (per + turn - 1u) / turn * turn;
     const uint32_t begin = split * per < sq.kv ? split * per : sq.kv;
     const uint32_t end = sq.kv - begin < per ? sq.kv : begin + per;
 
-    // This lane's query of each column tile.
-    uint32_t qv[NT][S::KP][4], node[NT];
-    size_t qwords[NT];              // its first word of the mask
+    // Queries: lane's column of each tile, as operands. Columns that are no query
+    // (past the rows) hold zeros, read from row 0.
+    uint4 qv[NT][S::KP];
+    uint32_t node[NT];
+    size_t qwords[NT];              // a query's first word of the mask
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        // Columns that are no query (past the rows) take row 0 and hold zeros.
         const uint32_t rr = rr0 + 16u * n + lm, nd = rr / a.group;
         const long long qrow = sq.row0 + nd;
         const bool live = rr < rows && qrow >= 0 && qrow < (long long)a.n_rows;
@@ -171,10 +225,8 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
 #pragma unroll
         for (int c = 0; c < S::KP; c++) {
             const uint4 x = *(const uint4 *)(p + 64u * c + 16u * lk);
-            qv[n][c][0] = live ? x.x : 0u;
-            qv[n][c][1] = live ? x.y : 0u;
-            qv[n][c][2] = live ? x.z : 0u;
-            qv[n][c][3] = live ? x.w : 0u;
+            qv[n][c] = uint4{live ? x.x ^ a.flip : 0u, live ? x.y ^ a.flip : 0u,
+                             live ? x.z ^ a.flip : 0u, live ? x.w ^ a.flip : 0u};
         }
     }
     float m[NT], l[NT];
@@ -193,7 +245,6 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
     const char *vbase = (const char *)a.v + (size_t)kvh * HD * sizeof(T);
     unsigned long long row[S::TILES];
     uint32_t nv[S::TILES];
-    uint32_t kr[S::TILES][S::KP][4], vr[S::TILES][4][S::VP][S::VD];
     auto find = [&](uint32_t c) {
 #pragma unroll
         for (int t = 0; t < S::TILES; t++) {
@@ -207,57 +258,47 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
             if (a.n_slots - r < nv[t]) nv[t] = (uint32_t)(a.n_slots - r);
         }
     };
-    // Rows past a tile's last are read as its last (of none, as row 0 of the
-    // cache).
-    auto load_k = [&]() {
+    // Copies of whole rows, 1 KiB each, from buffers that end with the tile's last
+    // row: rows past it are out of range, are not read and become zeros. 16-byte
+    // piece c of key k lies at place c ^ (k % 8), so that an operand's reads (one
+    // piece of 16 keys) meet no bank twice; values lie in order.
+    auto load = [&](const char *base, uint8_t *to, uint32_t turned) {
 #pragma unroll
-        for (int t = 0; t < S::TILES; t++) {
-            const uint32_t most = nv[t] ? nv[t] - 1u : 0u;
-            const char *p = kbase + row[t] * sb;
-            const uint32_t at = (lm < most ? lm : most) * sb + 16u * lk;
-#pragma unroll
-            for (int c = 0; c < S::KP; c++) load_dwords<4>(p + (at + 64u * c), kr[t][c]);
+        for (int j = 0; j < S::KB / 1024 / RW; j++) {
+            const uint32_t i = (uint32_t)(j * RW) + rw, at16 = i * S::RPI, first = at16 & 15u;
+            const bool low = S::TILES == 1 || at16 < 16u;
+            const uint32_t n = low ? nv[0] : nv[S::TILES - 1];
+            const unsigned long long r0 = low ? row[0] : row[S::TILES - 1];
+            const uint32_t at = __umul24(lane / S::CPR, sb) +
+                                16u * ((lane % S::CPR) ^ ((first + lane / S::CPR) & turned));
+            const uint32_t left = __builtin_amdgcn_readfirstlane((n > first ? n - first : 0u) * sb);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                __builtin_amdgcn_make_buffer_rsrc((void *)(base + (r0 + first) * sb), 0, left,
+                                                  0x00020000),
+                (ta_lds_void *)(to + 1024u * i), 16, at, 0, 0, 0);
         }
     };
-    auto load_v = [&]() {
+    // Lane's values: keys 4 lk + r of each tile, dimensions 16 CW c + CW lm + ...
+    uint32_t vr[S::TILES][4][S::VP][S::VD];
+    auto read_v = [&](const uint8_t *lds_v) {
 #pragma unroll
-        for (int t = 0; t < S::TILES; t++) {
-            const uint32_t most = nv[t] ? nv[t] - 1u : 0u;
-            const char *p = vbase + row[t] * sb;
+        for (int t = 0; t < S::TILES; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint32_t i = 4u * lk + r;
-                const uint32_t at = (i < most ? i : most) * sb + lm * (uint32_t)(S::CW * sizeof(T));
+            for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int c = 0; c < S::VP; c++)
-                    load_dwords<S::VD>(p + (at + c * (uint32_t)(16 * S::CW * sizeof(T))),
+                    load_dwords<S::VD>((const char *)lds_v +
+                                           (16u * t + 4u * lk + r) * (16u * S::CPR) +
+                                           (16u * c + lm) * (uint32_t)(S::CW * sizeof(T)),
                                        vr[t][r][c]);
-            }
-        }
     };
-    // Probabilities (lane's keys) as the second product's operand, and that
-    // product for tile e of the dimensions.
-    struct Probs { uint32_t d[4]; };
-    auto probs = [&](const float (&p)[S::TILES][4]) {
-        Probs o;
-        if constexpr (S::F32) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) o.d[r] = __float_as_uint(p[0][r]);
-        } else {
-            T h[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) h[j] = (T)p[j / 4][j % 4];
-            __builtin_memcpy(o.d, h, 16);
-        }
-        return o;
-    };
-    auto pv = [&](int e, const Probs &p, ta_v4f acc) {
+    auto pv = [&](int e, const uint32_t (&p)[4], ta_v4f acc) {
         const int c = e / S::CW;
         if constexpr (S::F32) {
 #pragma unroll
             for (int r = 0; r < 4; r++)
                 acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[0][r][c][e % 4]),
-                                                           __uint_as_float(p.d[r]), acc, 0, 0, 0);
+                                                           __uint_as_float(p[r]), acc, 0, 0, 0);
             return acc;
         } else {
             const int d = e % S::CW / 2;
@@ -268,127 +309,210 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
                 const int t = i / 2, r = 2 * (i & 1);
                 va[i] = __builtin_amdgcn_perm(vr[t][r + 1][c][d], vr[t][r][c][d], sel);
             }
-            return ta_mfma<T>(va, p.d, acc);
+            return ta_mfma<T>(va, p, acc);
         }
     };
-    bool bad = false;
 
-    uint32_t c = begin + wave * S::CK;
-    if (c < end) {
-        find(c);
-        load_k();
-        load_v();
-    }
-    while (c < end) {
-        const uint32_t next = c + S::CK * TA_WAVES;
-        uint32_t cnv[S::TILES];
-        bool whole = c + S::CK <= sq.past;
+    // Scores of the chunk in the registers: lane's query (column lm) against keys
+    // 4 lk + r of each tile.
+    float s[NT][S::TILES][4];
+    auto scores = [&](const uint8_t *lds_k) {
+        uint4 key[S::TILES][S::KP];
 #pragma unroll
-        for (int t = 0; t < S::TILES; t++) {
-            cnv[t] = nv[t];
-            whole = whole && nv[t] == 16u;
-        }
-        // Scores: lane's query (column lm) against keys 4 lk + r of each tile.
-        float s[NT][S::TILES][4];
+        for (int t = 0; t < S::TILES; t++)
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int k = 0; k < S::KP; k++)
+                key[t][k] = *(const uint4 *)(lds_k + (16u * t + lm) * (16u * S::CPR) +
+                                             16u * ((4u * k + lk) ^ (lm & 7u)));
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            uint4 q[S::KP];
+#pragma unroll
+            for (int k = 0; k < S::KP; k++) q[k] = qv[n][k];
 #pragma unroll
             for (int t = 0; t < S::TILES; t++) {
                 ta_v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < S::KP; k++) {
+                    const uint32_t qk[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+                    const uint32_t kk[4] = {key[t][k].x, key[t][k].y, key[t][k].z, key[t][k].w};
                     if constexpr (S::F32) {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
                             x = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                __uint_as_float(kr[t][k][i]), __uint_as_float(qv[n][k][i]), x, 0,
-                                0, 0);
+                                __uint_as_float(kk[i]), __uint_as_float(qk[i]), x, 0, 0, 0);
                     } else {
-                        x = ta_mfma<T>(kr[t][k], qv[n][k], x);
+                        x = ta_mfma<T>(kk, qk, x);
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < 4; r++) s[n][t][r] = x[r] * a.scale2;
+                for (int r = 0; r < 4; r++) s[n][t][r] = x[r];
             }
-        if (next < end) {
-            find(next);
-            load_k();
+            // One column tile after the other: their operands together would
+            // not fit the registers. And the copies that follow write where
+            // these keys were read.
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (!whole) {
-            // Unseen positions score -inf. Rows that are not there hold zeros,
-            // and so do a node's values that are not finite: 0 times them would
-            // be NaN in rows that do not see the node. They join at the end.
-#pragma unroll
-            for (int t = 0; t < S::TILES; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint32_t i = 4u * lk + r, p = c + 16u * t + i;
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        // Selected, not branched over: the compiler lost the
-                        // write of a branch here (ROCm 7.2, one f32 kernel).
-                        const uint32_t j = p < sq.past ? 0u : p - sq.past;
-                        const uint32_t ok =
-                            sees_node(a, qwords[n], node[n], j < sq.nodes ? j : sq.nodes - 1u) |
-                            (uint32_t)(p < sq.past);
-                        s[n][t][r] = (ok & (uint32_t)(i < cnv[t])) ? s[n][t][r] : -INFINITY;
-                    }
-#pragma unroll
-                    for (int x = 0; x < S::VP; x++)
-#pragma unroll
-                        for (int d = 0; d < S::VD; d++) {
-                            const bool odd = p >= sq.past && not_finite<T>(vr[t][r][x][d]);
-                            bad = bad || (odd && i < cnv[t]);
-                            if (i >= cnv[t]) vr[t][r][x][d] = 0u;
-                            else if (odd) vr[t][r][x][d] = finite_part<T>(vr[t][r][x][d]);
-                        }
-                }
-        }
-        Probs pr[NT];
+    };
+    // Their exponentials, and the values weighted by them.
+    auto weigh = [&]() {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            float top = -INFINITY;
+            float top = s[n][0][0];
 #pragma unroll
-            for (int t = 0; t < S::TILES; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) top = fmaxf(top, s[n][t][r]);
-            top = fmaxf(m[n], lane_max4(top));
-            const float base = top == -INFINITY ? 0.0f : top;
-            if (__any(top > m[n])) {
-                const float f = exp2_hw(m[n] - base);
+            for (int j = 1; j < 4 * S::TILES; j++) top = fmaxf(top, s[n][j / 4][j % 4]);
+            top *= a.scale2;
+            if (__any(top > m[n] + TA_LAG)) {
+                top = fmaxf(m[n], lane_max4(top));
+                const float f = exp2_hw(m[n] - (top == -INFINITY ? 0.0f : top));
                 l[n] *= f;
 #pragma unroll
                 for (int e = 0; e < S::VE; e++) o[n][e] *= f;
+                m[n] = top;
             }
-            m[n] = top;
-#pragma unroll
-            for (int t = 0; t < S::TILES; t++)
+            const float base = m[n] == -INFINITY ? 0.0f : m[n];
+            uint32_t p[4];
+            if constexpr (S::F32) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    s[n][t][r] = exp2_hw(s[n][t][r] - base);
-                    l[n] += s[n][t][r];
+                    const float x = exp2_hw(fmaf(s[n][0][r], a.scale2, -base));
+                    l[n] += x;
+                    p[r] = __float_as_uint(x);
                 }
-            pr[n] = probs(s[n]);
+            } else {
+                T h[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float x = exp2_hw(fmaf(s[n][j / 4][j % 4], a.scale2, -base));
+                    l[n] += x;
+                    h[j] = (T)x;
+                }
+                __builtin_memcpy(p, h, 16);
+            }
+#pragma unroll
+            for (int e = 0; e < S::VE; e++) o[n][e] = pv(e, p, o[n][e]);
+            if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    // Chunk c's keys and values are in flight or here (cnv: how many of each
+    // tile), the chunk after it is found (row, nv). Copies stand under no condition,
+    // so that the compiler keeps count of them in its waits (past the end they read
+    // nothing).
+    uint32_t c = begin + kg * S::CK, cnv[S::TILES];
+    auto advance = [&]() {
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int t = 0; t < S::TILES; t++) cnv[t] = nv[t];
+        find(c + turn);
+    };
+    // Whether its keys are all there and committed.
+    auto whole = [&]() {
+        bool w = c + S::CK <= sq.past && cnv[0] == 16u;
+        if constexpr (S::TILES > 1) w = w && cnv[1] == 16u;
+        return w;
+    };
+    // A chunk that is not whole (the nodes', the last, one with a bad page): unseen
+    // positions score -inf, and a node's values that are not finite become zeros, for
+    // 0 times them would be NaN in rows that do not see the node. They join at the end.
+    bool bad = false;
+    auto mask = [&]() {
 #pragma unroll
-            for (int e = 0; e < S::VE; e++) o[n][e] = pv(e, pr[n], o[n][e]);
-        if (next < end) load_v();
-        c = next;
+        for (int t = 0; t < S::TILES; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t i = 4u * lk + r, p = c + 16u * t + i;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    // Selected, not branched over: the compiler lost the write of
+                    // a branch here (ROCm 7.2, one f32 kernel).
+                    const uint32_t j = p < sq.past ? 0u : p - sq.past;
+                    const uint32_t ok =
+                        sees_node(a, qwords[n], node[n], j < sq.nodes ? j : sq.nodes - 1u) |
+                        (uint32_t)(p < sq.past);
+                    s[n][t][r] = (ok & (uint32_t)(i < cnv[t])) ? s[n][t][r] : -INFINITY;
+                }
+#pragma unroll
+                for (int x = 0; x < S::VP; x++)
+#pragma unroll
+                    for (int d = 0; d < S::VD; d++) {
+                        const uint32_t fit = finite_part<T>(vr[t][r][x][d]);
+                        const bool odd = p >= sq.past && fit != vr[t][r][x][d];
+                        bad = bad || odd;
+                        vr[t][r][x][d] = odd ? fit : vr[t][r][x][d];
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    find(c);
+    if constexpr (RW == 1) {
+        uint8_t *const k = kx + wave * S::KB, *const v = vx + wave * S::KB;
+        auto chunk = [&]() {
+            scores(k);
+            load(kbase, k, 7u);
+            read_v(v);
+            if (!whole()) mask();
+            weigh();
+            __builtin_amdgcn_sched_barrier(0);     // the values have been read
+            load(vbase, v, 0u);
+            c += turn;
+            advance();
+        };
+        load(kbase, k, 7u);
+        load(vbase, v, 0u);
+        advance();
+        while (c < end) chunk();
+    } else {
+        const uint32_t mine = kg * S::KB;
+        auto copy = [&](uint8_t *k, uint8_t *v) {
+            load(kbase, k + mine, 7u);
+            load(vbase, v + mine, 0u);
+        };
+        auto chunk = [&](const uint8_t *k, const uint8_t *v, uint8_t *next_k, uint8_t *next_v) {
+            // The chunk has landed, and everybody is done with the one before.
+            __builtin_amdgcn_s_waitcnt(0x0f70);    // vmcnt(0)
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            __builtin_amdgcn_sched_barrier(0);
+            copy(next_k, next_v);
+            scores(k + mine);
+            read_v(v + mine);
+            if (!whole()) mask();
+            weigh();
+            __builtin_amdgcn_sched_barrier(0);
+            c += turn;
+            advance();
+        };
+        copy(kx, vx);
+        advance();
+        // The same number of chunks, two by two, for every wave: past the end a chunk
+        // is empty.
+        for (uint32_t left = (end - begin + 2u * turn - 1u) / (2u * turn); left; left--) {
+            chunk(kx, vx, ky, vy);
+            chunk(ky, vy, kx, vx);
+        }
     }
 
     // The waves' sums meet, a column tile at a time.
+    // Place of dimension d (a multiple of 4, of the half in hand) of column `col` of
+    // wave w's results.
+    auto place = [&](uint32_t w, uint32_t col, uint32_t d) {
+        return (float *)kx + (16u * w + col) * (HD / 2) +
+               4u * ((d % (HD / 2) / 4u) ^ (col & 7u));
+    };
+    __builtin_amdgcn_s_waitcnt(0x0f70);                                 // no copy outlives the chunks' place
     if (__any(bad)) bad = true;
-    if (lane == 0) lbad[wave] = bad;
     const size_t heads_all = (size_t)a.n_rows * a.n_heads;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const float sum = lane_sum4(l[n]);
-        if (n) __syncthreads();
-        if (lk == 0) {
-            lm_[wave][lm] = m[n];
-            ll_[wave][lm] = sum;
+    for (int h = 0; h < 2 * NT; h++) {
+        const int n = h / 2;
+        __syncthreads();                           // the chunks' place, or the last half's
+        if (h % 2 == 0) {
+            const float sum = lane_sum4(l[n]);
+            if (lane == 0) lbad[wave] = bad;
+            if (lk == 0) {
+                lmax[wave][lm] = m[n];
+                lsum[wave][lm] = sum;
+            }
         }
         // Lane's dimensions: 16 CW c + CW (4 lk + r) + d.
 #pragma unroll
@@ -396,59 +520,68 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int d = 0; d < S::CW; d++)
-                    lo[wave][lm][16 * S::CW * x + S::CW * (4 * lk + r) + d] = o[n][x * S::CW + d][r];
+                for (int d = 0; d < S::CW; d += 4) {
+                    const uint32_t at = 16 * S::CW * x + S::CW * (4 * lk + r) + d;
+                    if (at / (HD / 2) == h % 2)
+                        *(float4 *)place(wave, lm, at) =
+                            float4{o[n][x * S::CW + d][r], o[n][x * S::CW + d + 1][r],
+                                   o[n][x * S::CW + d + 2][r], o[n][x * S::CW + d + 3][r]};
+                }
         __syncthreads();
-        // 16 threads a column, each every 16th run of four dimensions.
-        const uint32_t col = threadIdx.x >> 4, ln = threadIdx.x & 15u;
-        const uint32_t rr = rr0 + 16u * n + col, nd = rr / a.group;
-        const long long orow = sq.row0 + nd;
-        if (rr < rows && orow >= 0 && orow < (long long)a.n_rows) {
-            float top = -INFINITY, w[TA_WAVES], all = 0.0f;
+        // Each thread a run of four dimensions of a column.
+        for (uint32_t i = threadIdx.x; i < 2u * HD * RW; i += 64u * S::W) {
+            const uint32_t of = i / (2u * HD), col = i / (HD / 8u) % 16u;
+            const uint32_t d = i % (HD / 8u) * 4u + h % 2 * (HD / 2u);
+            const uint32_t rr = wg0 + 16u * (NT * of + n) + col, nd = rr / a.group;
+            const long long orow = sq.row0 + nd;
+            if (rr >= rows || orow < 0 || orow >= (long long)a.n_rows) continue;
+            float top = -INFINITY, all = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t any_bad = 0u;
 #pragma unroll
-            for (int i = 0; i < TA_WAVES; i++) top = fmaxf(top, lm_[i][col]);
+            for (int k = 0; k < KW; k++) {
+                top = fmaxf(top, lmax[RW * k + of][col]);
+                any_bad |= lbad[RW * k + of];
+            }
             const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int i = 0; i < TA_WAVES; i++) {
-                w[i] = exp2_hw(lm_[i][col] - base);
-                all = fmaf(w[i], ll_[i][col], all);
+            for (int k = 0; k < KW; k++) {
+                const uint32_t w = RW * k + of;
+                const float f = exp2_hw(lmax[w][col] - base);
+                const float4 x = *(const float4 *)place(w, col, d);
+                all = fmaf(f, lsum[w][col], all);
+                v[0] = fmaf(f, x.x, v[0]);
+                v[1] = fmaf(f, x.y, v[1]);
+                v[2] = fmaf(f, x.z, v[2]);
+                v[3] = fmaf(f, x.w, v[3]);
             }
             const uint32_t head = kvh * a.group + rr - nd * a.group;
-            const float inv = a.splits > 1u ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
-            const size_t at = split * heads_all + (size_t)orow * a.n_heads + head;
-            if (a.splits > 1u && ln == 0u) {
-                a.pm[at] = top;
-                a.pl[at] = all;
-            }
-            for (uint32_t d = 4u * ln; d < HD; d += 64u) {
-                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < TA_WAVES; i++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = fmaf(w[i], lo[i][col][d + k], v[k]);
-                if (lbad[0] | lbad[1] | lbad[2] | lbad[3]) {
-                    // Infinities and NaN of the nodes this row sees: whatever
-                    // their share, the sum becomes theirs.
-                    for (uint32_t p = sq.past > begin ? sq.past : begin; p < end; p++) {
-                        unsigned long long r;
-                        if (!sees_node(a, (size_t)orow * a.mask_words, nd, p - sq.past) ||
-                            !cache_row(a, b, p, r))
-                            continue;
-                        const T *x = (const T *)a.v + r * a.slot_stride + (size_t)kvh * HD + d;
-                        for (int k = 0; k < 4; k++) {
-                            const float y = (float)x[k];
-                            if (!(fabsf(y) < INFINITY)) v[k] += y;
-                        }
+            if (any_bad) {
+                // Infinities and NaN of the nodes this row sees: whatever their
+                // share, the sum becomes theirs.
+                for (uint32_t p = sq.past > begin ? sq.past : begin; p < end; p++) {
+                    unsigned long long r;
+                    if (!sees_node(a, (size_t)orow * a.mask_words, nd, p - sq.past) ||
+                        !cache_row(a, b, p, r))
+                        continue;
+                    const T *x = (const T *)a.v + r * a.slot_stride + (size_t)kvh * HD + d;
+                    for (int k = 0; k < 4; k++) {
+                        const float y = (float)x[k];
+                        if (!(fabsf(y) < INFINITY)) v[k] += y;
                     }
                 }
-                if (a.splits > 1u) {
-                    *(float4 *)(a.po + at * HD + d) = float4{v[0], v[1], v[2], v[3]};
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = all == 0.0f ? 0.0f : v[k] * inv;
-                    store4<true>((T *)a.out + (size_t)orow * a.out_stride + (size_t)head * HD + d,
-                                 v);
+            }
+            if (a.splits > 1u) {
+                const size_t at = split * heads_all + (size_t)orow * a.n_heads + head;
+                if (d == 0u) {
+                    a.pm[at] = top;
+                    a.pl[at] = all;
                 }
+                *(float4 *)(a.po + at * HD + d) = float4{v[0], v[1], v[2], v[3]};
+            } else {
+                const float inv = 1.0f / all;
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = all == 0.0f ? 0.0f : v[k] * inv;
+                store4<true>((T *)a.out + (size_t)orow * a.out_stride + (size_t)head * HD + d, v);
             }
         }
     }
@@ -466,44 +599,73 @@ MYNAH_DEV void tree_join(const TreeArgs &a) {
     if (nd >= sq.nodes || row < 0 || row >= (long long)a.n_rows || head >= a.n_heads) return;
     const size_t heads_all = (size_t)a.n_rows * a.n_heads;
     const size_t at = (size_t)row * a.n_heads + head;
+    // A split's maximum and sum to each lane, 64 of them at a time.
     float top = -INFINITY;
-    for (uint32_t s = 0; s < a.splits; s++) top = fmaxf(top, a.pm[s * heads_all + at]);
+    for (uint32_t s = lane; s < a.splits; s += 64u) top = fmaxf(top, a.pm[s * heads_all + at]);
+    top = wave_max_dpp(top);
     const float base = top == -INFINITY ? 0.0f : top;
     float all = 0.0f, v[E];
 #pragma unroll
     for (int i = 0; i < E; i++) v[i] = 0.0f;
-    for (uint32_t s = 0; s < a.splits; s++) {
-        const float w = exp2_hw(a.pm[s * heads_all + at] - base), ls = a.pl[s * heads_all + at];
-        all = fmaf(w, ls, all);
-        const float *p = a.po + (s * heads_all + at) * HD + E * lane;
+    for (uint32_t s0 = 0u; s0 < a.splits; s0 += 64u) {
+        const uint32_t n = a.splits - s0 < 64u ? a.splits - s0 : 64u;
+        const size_t from = (s0 + lane) * heads_all + at;
+        const float w = lane < n ? exp2_hw(a.pm[from] - base) : 0.0f;
+        all += lane < n ? w * a.pl[from] : 0.0f;
+        auto weight = [&](uint32_t s) {
+            return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
+        };
+        const float *p = a.po + (s0 * heads_all + at) * HD + E * lane;
+        uint32_t s = 0u;
+        for (; s + 8u <= n; s += 8u) {             // eight loads under way
+            float x[8][E];
 #pragma unroll
-        for (int i = 0; i < E; i++) v[i] = fmaf(w, p[i], v[i]);
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int i = 0; i < E; i++) x[j][i] = p[(s + j) * heads_all * HD + i];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int i = 0; i < E; i++) v[i] = fmaf(weight(s + j), x[j][i], v[i]);
+        }
+        for (; s < n; s++)
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] = fmaf(weight(s), p[s * heads_all * HD + i], v[i]);
     }
+    all = wave_sum(all);
     T *y = (T *)a.out + (size_t)row * a.out_stride + (size_t)head * HD + E * lane;
 #pragma unroll
     for (int i = 0; i < E; i++) y[i] = (T)(all == 0.0f ? 0.0f : v[i] / all);
 }
 
-#define TREE_KERNEL(name, T, HD, NT, W)                                                  \
-    extern "C" __global__ void __launch_bounds__(64 * TA_WAVES, W)                       \
-        mynah_tree_attn_##name##_##HD##_##NT(TreeArgs a) { tree_attn<T, HD, NT>(a); }
+#define TREE_KERNEL(name, T, HD, NT, RW)                                                 \
+    extern "C" __global__ void __launch_bounds__((64 * TaShape<T, HD>::W),               \
+                                                 (TaShape<T, HD>::W / 4))                \
+        mynah_tree_attn_##name##_##HD##_##NT##x##RW(TreeArgs a) {                        \
+        tree_attn<T, HD, NT, RW>(a);                                                     \
+    }
 #define TREE_JOIN(name, T, HD)                                                           \
     extern "C" __global__ void __launch_bounds__(256) mynah_tree_join_##name##_##HD(     \
         TreeArgs a) { tree_join<T, HD>(a); }
+TREE_KERNEL(f32, float, 64, 1, 1)
 TREE_KERNEL(f32, float, 64, 1, 2)
-TREE_KERNEL(f32, float, 64, 2, 2)
+TREE_KERNEL(f32, float, 128, 1, 1)
 TREE_KERNEL(f32, float, 128, 1, 2)
-TREE_KERNEL(f32, float, 128, 2, 2)
 TREE_KERNEL(f32, float, 256, 1, 1)
-#define TREE_KERNELS16(name, T)   \
+TREE_KERNEL(f32, float, 256, 1, 2)
+#define TREE_KERNELS16(name, T) \
+    TREE_KERNEL(name, T, 64, 1, 1)  \
     TREE_KERNEL(name, T, 64, 1, 2)  \
     TREE_KERNEL(name, T, 64, 2, 2)  \
-    TREE_KERNEL(name, T, 64, 4, 2)  \
+    TREE_KERNEL(name, T, 64, 2, 4)  \
+    TREE_KERNEL(name, T, 128, 1, 1) \
     TREE_KERNEL(name, T, 128, 1, 2) \
     TREE_KERNEL(name, T, 128, 2, 2) \
-    TREE_KERNEL(name, T, 128, 4, 1) \
+    TREE_KERNEL(name, T, 128, 2, 4) \
+    TREE_KERNEL(name, T, 128, 2, 8) \
     TREE_KERNEL(name, T, 256, 1, 1) \
-    TREE_KERNEL(name, T, 256, 2, 1)
+    TREE_KERNEL(name, T, 256, 1, 2) \
+    TREE_KERNEL(name, T, 256, 1, 4)
 TREE_KERNELS16(f16, _Float16)
 TREE_KERNELS16(bf16, __bf16)
 TREE_JOIN(f32, float, 64)

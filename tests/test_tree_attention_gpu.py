@@ -165,6 +165,15 @@ def test_long_context_and_equal_bits(M, t):
     assert np.array_equal(a.view(np.uint8), c.call().view(np.uint8))
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_more_splits_than_lanes(M, t, hd):
+    # One key head: its positions go to every CU, and more than 64 sums meet in a wave.
+    c = Tree(M, [(29_989, 3)], 4, 1, hd, t, seed=5)
+    assert M.tree_attention_workspace(c.args()) > 65 * 12 * (hd + 2) * 4
+    c.check(c.call())
+
+
 def test_one_workspace_byte_short(M):
     c = Tree(M, [(900, 2)], 4, 1, 128, E.F32)
     a = c.args()
