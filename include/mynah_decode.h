@@ -91,6 +91,34 @@ int mynah_hip_qwen3_prompt(mynah_qwen3 *s, const uint32_t *prompt, uint32_t n_pr
  * matvec's. 0, or -1 when the tokens do not fit the context. */
 int mynah_hip_qwen3_prefill(mynah_qwen3 *s, const uint32_t *tokens, uint32_t n);
 
+/* One verification step of drafted tokens (no reference counterpart: the
+ * reference decodes one token at a time, src/generate.c:47-77): n nodes, 1 to
+ * MYNAH_MAX_DRAFT, of a tree. Node i holds tokens[i] and follows node
+ * parents[i] < i, or with -1 the last cached position; parents NULL is a chain.
+ * It stands at position n_past + its depth and attends the cached positions, its
+ * ancestors and itself. greedy_out[i] receives the greedy choice after node i
+ * (src/sampler.c:122-129), logits (optional, host) its [n][vocab] logits; both
+ * differ from those that mynah_hip_qwen3_forward gives along the node's path by
+ * f32 rounding only. The nodes' keys and values stand in the cache rows behind
+ * n_past, which stays as it was, until mynah_hip_qwen3_accept keeps some of them or
+ * another call writes there. 0, or -1 with the reason in mynah_hip_last_error(). */
+enum { MYNAH_MAX_DRAFT = 256 };
+int mynah_hip_qwen3_verify(mynah_qwen3 *s, const uint32_t *tokens, const int32_t *parents,
+                           uint32_t n, uint32_t *greedy_out, float *logits);
+
+/* Keep a path of the last verify's nodes: nodes[0] without a parent, every other
+ * one the child of the one before. Their rows move up to n_past, which advances by
+ * count; the other nodes are gone. -1 and no change where the nodes are no path or
+ * another call than verify has come between. */
+int mynah_hip_qwen3_accept(mynah_qwen3 *s, const uint32_t *nodes, uint32_t count);
+
+/* Drop n cached positions from `first` on (no reference counterpart: the
+ * reference's context ends when it is full): later ones move down by n, their
+ * keys rotated back by n positions, and n_past becomes n_past - n. first + n =
+ * n_past takes the last n positions back. What the moved keys and values hold of
+ * the dropped tokens' content stays in them. */
+int mynah_hip_qwen3_drop(mynah_qwen3 *s, uint32_t first, uint32_t n);
+
 /* How mynah_hip_qwen3_prompt fills the cache with the prompt:
  *   MYNAH_PREFILL_BATCHED (default): mynah_hip_qwen3_prefill;
  *   MYNAH_PREFILL_STEPS: one decode step per token, in the current GEMV

@@ -25,6 +25,7 @@
  * SPDX-License-Identifier: MIT */
 #define _GNU_SOURCE
 #include "kernels_hip.h"
+#include "mynah_attention.h"
 #include "mynah_decode.h"
 #include "mynah_generate.h"
 #include "runtime_internal.h"
@@ -115,6 +116,22 @@ struct mynah_qwen3 {
      * sampler for the length of a generation) and its scratch. */
     SampState *samp_st;
     samp_scratch samp_sc;
+    /* Verification of drafted tokens (allocated on first use for dr_cap nodes, the
+     * attention's workspace for dr_ws_bytes): activations as in the prefill,
+     * queries before and after norm and rotation, keys and values on their way to the
+     * cache, logits, and the integers of a call (dr_int: see draft_ints). */
+    uint32_t dr_cap;
+    float *dr_x, *dr_xn, *dr_q, *dr_qr, *dr_k, *dr_v, *dr_g, *dr_u, *dr_logits;
+    int32_t *dr_int;
+    void *dr_ws;
+    size_t dr_ws_bytes;
+    double *rope_freqs;             /* radians per position of each pair */
+    float *drop_rows;               /* rows on their way down (mynah_hip_qwen3_drop) */
+    int32_t *drop_pos;
+    /* The nodes whose rows stand behind n_past, waiting for an accept; 0 once
+     * anything else has written the cache. */
+    uint32_t draft_n;
+    int32_t draft_parent[MYNAH_MAX_DRAFT];
 };
 
 #define TOKEN(s) ((s)->counters + 0)
@@ -208,7 +225,9 @@ void mynah_hip_qwen3_free(mynah_qwen3 *s) {
                     s->x, s->q, s->k_now,
                     s->attn, s->act, s->logits, s->scores, s->counters, s->tokens, s->forced, s->pm, s->pl,
                     s->po, s->pf_x, s->pf_xn, s->pf_q, s->pf_att, s->pf_g, s->pf_u, s->pf_s,
-                    s->pf_tok};
+                    s->pf_tok, s->dr_x, s->dr_xn, s->dr_q, s->dr_qr, s->dr_k, s->dr_v, s->dr_g,
+                    s->dr_u, s->dr_logits, s->dr_int, s->dr_ws, s->rope_freqs, s->drop_rows,
+                    s->drop_pos};
     for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++)
         if (bufs[i]) (void)hipFree(bufs[i]);
     if (s->host_logits) (void)hipHostFree(s->host_logits);
@@ -818,6 +837,7 @@ static uint32_t ensure_graph(mynah_qwen3 *s, mynah_device *d, int v, uint32_t p0
 /* One launch of variant v starting at position p0: its bucket's graph, or
  * direct launches without one. */
 static int run_step(mynah_qwen3 *s, mynah_device *d, int v, uint32_t p0) {
+    s->draft_n = 0;
     hipStream_t st = d->stream;
     const uint32_t b = ensure_graph(s, d, v, p0);
     if (s->graph_state[v][b] == 1) {
@@ -977,6 +997,7 @@ static int enqueue_prefill_chunk(mynah_qwen3 *s, mynah_device *d, hipStream_t st
     const size_t per_layer = (size_t)s->n_ctx * s->kv_dim;
     uint32_t p0 = s->n_past, dm = c->d_model;
     const uint32_t group = c->n_heads / c->n_kv_heads;
+    s->draft_n = 0;
     int rc;
     {
         const unsigned char *tab = s->embed.dev;
@@ -1121,6 +1142,375 @@ int mynah_hip_qwen3_prefill(mynah_qwen3 *s, const uint32_t *tokens, uint32_t n) 
         mynah_set_error("prefill failed");
         return -1;
     }
+    return 0;
+}
+
+/* ── verification of drafted tokens ──────────────────────────────────────── */
+
+/* The integers of a call, in one upload: tokens, positions and cache rows of the
+ * nodes, the sequence's row range and its committed positions, the mask. The
+ * greedy choices come back in their own place, accept's path goes to the
+ * tokens'. */
+typedef struct {
+    int32_t *tokens, *pos, *slots, *greedy, *start, *past;
+    uint32_t *mask;
+} draft_ints;
+
+static size_t draft_count(uint32_t cap) { return 4 * (size_t)cap + 4 + (size_t)cap * (cap / 32); }
+
+static draft_ints draft_lay_out(int32_t *at, uint32_t cap) {
+    draft_ints v;
+    v.tokens = at;
+    v.pos = v.tokens + cap;
+    v.slots = v.pos + cap;
+    v.start = v.slots + cap;
+    v.past = v.start + 2;
+    v.mask = (uint32_t *)(v.past + 2);
+    v.greedy = (int32_t *)(v.mask + (size_t)cap * (cap / 32));
+    return v;
+}
+
+static int rope_table(mynah_qwen3 *s) {
+    if (s->rope_freqs != NULL) return 0;
+    const uint32_t half = s->c.head_dim / 2;
+    double *f = (double *)malloc(half * sizeof *f);
+    float mscale;
+    const mynah_rope_params p = {.rot_dim = s->c.head_dim, .theta = (double)s->c.rope_theta};
+    int ok = f != NULL && mynah_hip_rope_freqs(&p, f, &mscale) == 0;
+    if (ok) s->rope_freqs = (double *)dalloc(half * sizeof *f, &ok);
+    if (ok && hipMemcpy(s->rope_freqs, f, half * sizeof *f, hipMemcpyHostToDevice) != hipSuccess) {
+        (void)hipFree(s->rope_freqs);
+        s->rope_freqs = NULL;
+        ok = 0;
+    }
+    free(f);
+    if (!ok) mynah_set_error("no table of rotary frequencies");
+    return ok ? 0 : -1;
+}
+
+static int draft_alloc(mynah_qwen3 *s, uint32_t n) {
+    if (rope_table(s) != 0) return -1;
+    if (s->dr_cap >= n) return 0;
+    const uint32_t cap = (n + 31u) & ~31u;
+    const mynah_qwen3_shape *c = &s->c;
+    int ok = 1;
+    s->dr_cap = 0;
+    struct {
+        void **at;
+        size_t bytes;
+    } bufs[] = {{(void **)&s->dr_x, (size_t)cap * c->d_model * 4},
+                {(void **)&s->dr_xn, (size_t)cap * c->d_model * 4},
+                {(void **)&s->dr_q, (size_t)cap * s->q_dim * 4},
+                {(void **)&s->dr_qr, (size_t)cap * s->q_dim * 4},
+                {(void **)&s->dr_k, (size_t)cap * s->kv_dim * 4},
+                {(void **)&s->dr_v, (size_t)cap * s->kv_dim * 4},
+                {(void **)&s->dr_g, (size_t)cap * c->d_ff * 4},
+                {(void **)&s->dr_u, (size_t)cap * c->d_ff * 4},
+                {(void **)&s->dr_logits, (size_t)cap * c->vocab * 4},
+                {(void **)&s->dr_int, draft_count(cap) * 4}};
+    for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) {
+        if (*bufs[i].at) (void)hipFree(*bufs[i].at);
+        *bufs[i].at = dalloc(bufs[i].bytes, &ok);
+    }
+    if (!ok) {
+        mynah_set_error("out of device memory for %u drafted tokens", cap);
+        return -1;
+    }
+    s->dr_cap = cap;
+    return 0;
+}
+
+/* Every layer over the n nodes in dr_int, then the head. */
+static int enqueue_draft(mynah_qwen3 *s, mynah_device *d, hipStream_t st, uint32_t n,
+                         const draft_ints *v) {
+    const mynah_qwen3_shape *c = &s->c;
+    const size_t per_layer = (size_t)s->n_ctx * s->kv_dim;
+    uint32_t dm = c->d_model;
+    float eps = c->rms_eps;
+    int rc;
+    {
+        const unsigned char *tab = s->embed.dev;
+        const int32_t *tk = v->tokens;
+        float *x = s->dr_x;
+        uint32_t ty = (uint32_t)s->embed.type, rb = (uint32_t)s->embed.row_bytes;
+        void *args[] = {&tab, &tk, &x, &dm, &ty, &rb};
+        rc = mynah_launch(d, MYNAH_K_EMBED_ROWS, (dm / 32 + 255) / 256, n, 256, 0, st, args);
+    }
+#define NORM_ROWS(weight, threads)                                                         \
+    do {                                                                                   \
+        const float *x = s->dr_x, *w = (const float *)(weight).dev;                        \
+        float *o = s->dr_xn;                                                               \
+        void *args[] = {&x, &w, &o, &dm, &eps};                                            \
+        rc = rc ? rc : mynah_launch(d, MYNAH_K_RMSNORM_ROWS, n, 1, threads, 0, st, args);  \
+    } while (0)
+#define PRODUCT(w, from, to, res)                                                          \
+    rc = rc ? rc : mynah_matmat_mv_launch(d, (w).type, (w).dev, (w).rows, (w).cols, from,  \
+                                          to, n, res, st)
+    for (uint32_t l = 0; l < c->n_layers && rc == 0; l++) {
+        const dlayer *L = &s->layers[l];
+        float *kl = s->k_cache + l * per_layer, *vl = s->v_cache + l * per_layer;
+        uint32_t thr_attn = 0, thr_ffn = 0;
+        rc = norm_threads(s, L, 0, &thr_attn);
+        rc = rc ? rc : norm_threads(s, L, 1, &thr_ffn);
+        if (rc) break;
+        NORM_ROWS(L->attn_norm, thr_attn);
+        PRODUCT(L->wq, s->dr_xn, s->dr_q, NULL);
+        PRODUCT(L->wk, s->dr_xn, s->dr_k, NULL);
+        PRODUCT(L->wv, s->dr_xn, s->dr_v, NULL);
+        const mynah_qk_norm_rope qk = {
+            .type = MYNAH_F32, .out_type = MYNAH_F32, .layout = MYNAH_ROPE_HALF,
+            .n_heads = c->n_heads, .n_kv_heads = c->n_kv_heads, .head_dim = c->head_dim,
+            .rot_dim = c->head_dim, .tokens = n, .q = s->dr_q, .k = s->dr_k, .v = s->dr_v,
+            .q_stride = s->q_dim, .k_stride = s->kv_dim, .v_stride = s->kv_dim,
+            .q_norm = (const float *)L->q_norm.dev, .k_norm = (const float *)L->k_norm.dev,
+            .eps = eps, .mscale = 1.0f, .freqs = s->rope_freqs, .pos = v->pos,
+            .slots = v->slots, .n_slots = s->n_ctx, .q_out = s->dr_qr,
+            .q_out_stride = s->q_dim, .k_cache = kl, .v_cache = vl, .slot_stride = s->kv_dim};
+        rc = rc ? rc : mynah_hip_qk_norm_rope_dev(&qk, st);
+        const mynah_tree_attention at = {
+            .type = MYNAH_F32, .n_seqs = 1, .n_heads = c->n_heads,
+            .n_kv_heads = c->n_kv_heads, .head_dim = c->head_dim, .q = s->dr_qr,
+            .q_stride = s->q_dim, .out = s->dr_q, .out_stride = s->q_dim, .n_rows = n,
+            .k_cache = kl, .v_cache = vl, .slot_stride = s->kv_dim, .n_slots = s->n_ctx,
+            .seq_slots = s->n_ctx, .seq_start = v->start, .n_past = v->past, .mask = v->mask,
+            .mask_words = s->dr_cap / 32, .max_nodes = n, .max_kv = s->n_past + n,
+            .scale = s->scale};
+        if (rc == 0 && l == 0) {
+            const size_t need = mynah_hip_tree_attention_workspace(&at);
+            if (need == 0) return -1;
+            if (need > s->dr_ws_bytes) {
+                int ok = 1;
+                if (s->dr_ws) (void)hipFree(s->dr_ws);
+                s->dr_ws_bytes = 0;
+                s->dr_ws = dalloc(need, &ok);
+                if (!ok) {
+                    mynah_set_error("out of device memory for the attention's workspace");
+                    return -1;
+                }
+                s->dr_ws_bytes = need;
+            }
+        }
+        rc = rc ? rc : mynah_hip_tree_attention_dev(&at, s->dr_ws, s->dr_ws_bytes, st);
+        PRODUCT(L->wo, s->dr_q, s->dr_x, s->dr_x);
+        NORM_ROWS(L->ffn_norm, thr_ffn);
+        PRODUCT(L->gate, s->dr_xn, s->dr_g, NULL);
+        PRODUCT(L->up, s->dr_xn, s->dr_u, NULL);
+        if (rc == 0) {
+            const float *g = s->dr_g, *u = s->dr_u;
+            float *a = s->dr_g;
+            uint32_t count = n * c->d_ff;
+            void *args[] = {&g, &u, &a, &count};
+            rc = mynah_launch(d, MYNAH_K_SWIGLU_ROWS, (count + 255) / 256, 1, 256, 0, st, args);
+        }
+        PRODUCT(L->down, s->dr_g, s->dr_x, s->dr_x);
+    }
+    mynah_gemv_group hg;
+    uint32_t thr = 0;
+    rc = rc ? rc : head_group(s, &hg);
+    rc = rc ? rc : mynah_gemv_group_threads(&hg, MYNAH_GEMV_EXACT, &thr);
+    NORM_ROWS(s->out_norm, thr);
+    PRODUCT(s->head, s->dr_xn, s->dr_logits, NULL);
+#undef PRODUCT
+#undef NORM_ROWS
+    if (rc == 0) {
+        const float *lg = s->dr_logits;
+        uint32_t vocab = c->vocab;
+        int32_t *ids = v->greedy;
+        void *args[] = {&lg, &vocab, &ids};
+        rc = mynah_launch(d, MYNAH_K_ARGMAX_ROWS, n, 1, 1024, 0, st, args);
+    }
+    return rc;
+}
+
+int mynah_hip_qwen3_verify(mynah_qwen3 *s, const uint32_t *tokens, const int32_t *parents,
+                           uint32_t n, uint32_t *greedy_out, float *logits) {
+    if (s == NULL || tokens == NULL || greedy_out == NULL) {
+        mynah_set_error("verify: null argument");
+        return -1;
+    }
+    if (n == 0 || n > MYNAH_MAX_DRAFT) {
+        mynah_set_error("verify: %u nodes, 1 to %u are taken", n, MYNAH_MAX_DRAFT);
+        return -1;
+    }
+    if (n > s->n_ctx - s->n_past) {
+        mynah_set_error("verify: %u nodes do not fit the context (%u of %u used)", n, s->n_past,
+                        s->n_ctx);
+        return -1;
+    }
+    for (uint32_t i = 0; i < n; i++) {
+        if (tokens[i] >= s->c.vocab) {
+            mynah_set_error("token %u out of range", tokens[i]);
+            return -1;
+        }
+        if (parents != NULL && (parents[i] < -1 || parents[i] >= (int64_t)i)) {
+            mynah_set_error("verify: node %u has parent %d, -1 or an earlier node is needed", i,
+                            parents[i]);
+            return -1;
+        }
+    }
+    mynah_device *d = mynah_dev();
+    if (d == NULL) return -1;
+    s->draft_n = 0;
+    if (draft_alloc(s, n) != 0) return -1;
+    const draft_ints dev = draft_lay_out(s->dr_int, s->dr_cap);
+    const uint32_t words = s->dr_cap / 32;
+    int32_t *host = (int32_t *)calloc(draft_count(s->dr_cap), sizeof *host);
+    if (host == NULL) {
+        mynah_set_error("out of memory");
+        return -1;
+    }
+    const draft_ints v = draft_lay_out(host, s->dr_cap);
+    for (uint32_t i = 0; i < n; i++) {
+        const int32_t p = parents != NULL ? parents[i] : (int32_t)i - 1;
+        s->draft_parent[i] = p;
+        v.tokens[i] = (int32_t)tokens[i];
+        v.pos[i] = p < 0 ? (int32_t)s->n_past : v.pos[p] + 1;
+        v.slots[i] = (int32_t)(s->n_past + i);
+        if (p >= 0) memcpy(v.mask + (size_t)i * words, v.mask + (size_t)p * words, words * 4);
+        v.mask[(size_t)i * words + i / 32] |= 1u << (i % 32);
+    }
+    v.start[1] = (int32_t)n;
+    v.past[0] = (int32_t)s->n_past;
+    hipStream_t st = d->stream;
+    int rc = 0;
+    if (hipMemcpyAsync(s->dr_int, host, draft_count(s->dr_cap) * 4, hipMemcpyHostToDevice, st) !=
+        hipSuccess) {
+        mynah_set_error("verify: upload failed");
+        rc = -1;
+    }
+    rc = rc ? rc : enqueue_draft(s, d, st, n, &dev);
+    if (rc == 0 && (hipMemcpyAsync(greedy_out, dev.greedy, (size_t)n * 4, hipMemcpyDeviceToHost,
+                                   st) != hipSuccess ||
+                    (logits != NULL &&
+                     hipMemcpyAsync(logits, s->dr_logits, (size_t)n * s->c.vocab * 4,
+                                    hipMemcpyDeviceToHost, st) != hipSuccess))) {
+        mynah_set_error("verify: download failed");
+        rc = -1;
+    }
+    if (hipStreamSynchronize(st) != hipSuccess && rc == 0) {
+        mynah_set_error("verify failed");
+        rc = -1;
+    }
+    free(host);                     /* no copy reads it any more */
+    if (rc == 0) s->draft_n = n;
+    return rc;
+}
+
+int mynah_hip_qwen3_accept(mynah_qwen3 *s, const uint32_t *nodes, uint32_t count) {
+    if (s == NULL || (nodes == NULL && count != 0)) {
+        mynah_set_error("accept: null argument");
+        return -1;
+    }
+    if (count > s->draft_n) {
+        mynah_set_error("accept: %u nodes, %u wait", count, s->draft_n);
+        return -1;
+    }
+    uint32_t moved = 0;
+    for (uint32_t i = 0; i < count; i++) {
+        if (nodes[i] >= s->draft_n ||
+            s->draft_parent[nodes[i]] != (i ? (int32_t)nodes[i - 1] : -1)) {
+            mynah_set_error("accept: node %u does not follow the one before", nodes[i]);
+            return -1;
+        }
+        moved += nodes[i] != i;
+    }
+    mynah_device *d = mynah_dev();
+    if (d == NULL) return -1;
+    if (moved != 0) {
+        hipStream_t st = d->stream;
+        float *k = s->k_cache, *v = s->v_cache;
+        const int32_t *path = s->dr_int;
+        uint32_t base = s->n_past, kvd = s->kv_dim;
+        size_t per_layer = (size_t)s->n_ctx * s->kv_dim;
+        void *args[] = {&k, &v, &path, &count, &base, &kvd, &per_layer};
+        if (hipMemcpyAsync(s->dr_int, nodes, (size_t)count * 4, hipMemcpyHostToDevice, st) !=
+                hipSuccess ||
+            mynah_launch3(d, MYNAH_K_KV_COMPACT, (kvd + 255) / 256, s->c.n_layers, 2, 64, 0, st,
+                          args) != 0 ||
+            hipStreamSynchronize(st) != hipSuccess) {
+            mynah_set_error("accept failed");
+            s->draft_n = 0;
+            return -1;
+        }
+    }
+    s->n_past += count;
+    s->draft_n = 0;
+    return 0;
+}
+
+/* Rows on their way down at a time: what is written ends below what is still to
+ * be read, whatever their number. */
+#define DROP_ROWS 4096u
+
+int mynah_hip_qwen3_drop(mynah_qwen3 *s, uint32_t first, uint32_t n) {
+    if (s == NULL) {
+        mynah_set_error("drop: null argument");
+        return -1;
+    }
+    if (first > s->n_past || n > s->n_past - first) {
+        mynah_set_error("drop: positions %u .. %u + %u of %u", first, first, n, s->n_past);
+        return -1;
+    }
+    mynah_device *d = mynah_dev();
+    if (d == NULL) return -1;
+    s->draft_n = 0;
+    const uint32_t later = s->n_past - first - n;
+    if (n != 0 && later != 0) {
+        const mynah_qwen3_shape *c = &s->c;
+        int ok = rope_table(s) == 0;
+        if (!ok) return -1;
+        if (s->drop_rows == NULL) {
+            const uint32_t most = s->n_ctx < DROP_ROWS ? s->n_ctx : DROP_ROWS;
+            s->drop_rows = (float *)dalloc((size_t)most * s->kv_dim * 4, &ok);
+            if (ok && s->drop_pos == NULL) s->drop_pos = (int32_t *)dalloc((size_t)most * 4, &ok);
+            if (!ok) {
+                if (s->drop_rows) (void)hipFree(s->drop_rows);
+                s->drop_rows = NULL;
+                mynah_set_error("out of device memory for the moved rows");
+                return -1;
+            }
+        }
+        const uint32_t most = later < DROP_ROWS ? later : DROP_ROWS;
+        int32_t *back = (int32_t *)malloc((size_t)most * 4);
+        if (back == NULL) {
+            mynah_set_error("out of memory");
+            return -1;
+        }
+        for (uint32_t i = 0; i < most; i++) back[i] = -(int32_t)n;
+        hipStream_t st = d->stream;
+        int rc = hipMemcpyAsync(s->drop_pos, back, (size_t)most * 4, hipMemcpyHostToDevice, st) ==
+                         hipSuccess ? 0 : -1;
+        const size_t row = (size_t)s->kv_dim, per_layer = (size_t)s->n_ctx * row;
+        for (uint32_t at = 0; at < later && rc == 0; at += DROP_ROWS) {
+            const uint32_t m = later - at < DROP_ROWS ? later - at : DROP_ROWS;
+            const size_t bytes = (size_t)m * row * 4;
+            for (uint32_t l = 0; l < c->n_layers && rc == 0; l++) {
+                float *k = s->k_cache + l * per_layer + (first + at) * row;
+                float *v = s->v_cache + l * per_layer + (first + at) * row;
+                rc = mynah_hip_rope_dev(MYNAH_F32, MYNAH_ROPE_HALF, k + n * row, row, c->head_dim,
+                                        s->drop_rows, row, c->head_dim, m, c->n_kv_heads,
+                                        c->head_dim, c->head_dim, s->rope_freqs, 1.0f,
+                                        s->drop_pos, st);
+                if (rc == 0 &&
+                    (hipMemcpyAsync(k, s->drop_rows, bytes, hipMemcpyDeviceToDevice, st) !=
+                         hipSuccess ||
+                     hipMemcpyAsync(s->drop_rows, v + n * row, bytes, hipMemcpyDeviceToDevice,
+                                    st) != hipSuccess ||
+                     hipMemcpyAsync(v, s->drop_rows, bytes, hipMemcpyDeviceToDevice, st) !=
+                         hipSuccess))
+                    rc = -1;
+            }
+        }
+        if (hipStreamSynchronize(st) != hipSuccess) rc = -1;
+        free(back);
+        if (rc != 0) {
+            /* Some rows are moved, some are not: nothing of them is kept. */
+            mynah_set_error("drop failed, positions from %u on are lost", first);
+            s->n_past = first;
+            return -1;
+        }
+    }
+    s->n_past -= n;
     return 0;
 }
 
@@ -1652,6 +2042,7 @@ int mynah_hip_qwen3_set_kv(mynah_qwen3 *s, const float *k, const float *v, uint3
         mynah_set_error("bad KV prefill");
         return -1;
     }
+    s->draft_n = 0;
     const size_t row = (size_t)n_pos * s->kv_dim, per_layer = (size_t)s->n_ctx * s->kv_dim;
     for (uint32_t l = 0; l < s->c.n_layers; l++) {
         if (hipMemcpy(s->k_cache + l * per_layer, k + l * row, row * 4, hipMemcpyHostToDevice) != hipSuccess ||
@@ -1703,7 +2094,9 @@ int mynah_hip_qwen3_read_attn(const mynah_qwen3 *s, float *out) {
 }
 
 void mynah_hip_qwen3_reset(mynah_qwen3 *s) {
-    if (s) s->n_past = 0;
+    if (s == NULL) return;
+    s->n_past = 0;
+    s->draft_n = 0;
 }
 
 int mynah_hip_qwen3_uses_graph(const mynah_qwen3 *s) {

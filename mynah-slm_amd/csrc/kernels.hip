@@ -17,3 +17,4 @@
 #include "rope.hip"
 #include "fp8.hip"
 #include "tree_attn.hip"
+#include "draft.hip"

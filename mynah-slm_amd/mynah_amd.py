@@ -190,6 +190,9 @@ def _load() -> C.CDLL:
         "mynah_hip_qwen3_set_kv": (C.c_int, [_P, _P, _P, C.c_uint32]),
         "mynah_hip_qwen3_get_kv": (C.c_int, [_P, _P, _P, C.c_uint32]),
         "mynah_hip_qwen3_prefill": (C.c_int, [_P, _P, C.c_uint32]),
+        "mynah_hip_qwen3_verify": (C.c_int, [_P, _P, _P, C.c_uint32, _P, _P]),
+        "mynah_hip_qwen3_accept": (C.c_int, [_P, _P, C.c_uint32]),
+        "mynah_hip_qwen3_drop": (C.c_int, [_P, C.c_uint32, C.c_uint32]),
         "mynah_hip_qwen3_set_prefill": (C.c_int, [_P, C.c_int]),
         "mynah_hip_qwen3_n_past": (C.c_uint32, [_P]),
         "mynah_hip_qwen3_read_attn": (C.c_int, [_P, _P]),
@@ -784,6 +787,29 @@ class Qwen3Decoder:
         (bit-identical to one forward(token, want_logits=False) per token)."""
         p = np.ascontiguousarray(tokens, dtype=np.uint32)
         check(lib.mynah_hip_qwen3_prefill(self.h, ptr(p), p.size), "prefill")
+
+    def verify(self, tokens, parents=None, want_logits: bool = False):
+        """One step over drafted tokens (a tree by `parents`, -1 for none; a chain
+        without): the greedy id after each, and its logits [n][vocab] on request.
+        The position stays until accept()."""
+        t = np.ascontiguousarray(tokens, dtype=np.uint32)
+        p = None if parents is None else np.ascontiguousarray(parents, dtype=np.int32)
+        if t.ndim != 1 or (p is not None and p.shape != t.shape):
+            raise ValueError("verify: one parent for each token")
+        ids = np.empty(t.size, np.uint32)
+        logits = np.empty((t.size, self.model.shape.vocab), np.float32) if want_logits else None
+        check(lib.mynah_hip_qwen3_verify(self.h, ptr(t), None if p is None else ptr(p), t.size,
+                                         ptr(ids), ptr(logits) if want_logits else None), "verify")
+        return (ids, logits) if want_logits else ids
+
+    def accept(self, nodes) -> None:
+        """Keep a path of the last verify()'s nodes."""
+        p = np.ascontiguousarray(nodes, dtype=np.uint32)
+        check(lib.mynah_hip_qwen3_accept(self.h, ptr(p), p.size), "accept")
+
+    def drop(self, first: int, n: int) -> None:
+        """Take n cached positions from `first` on out; later ones move down."""
+        check(lib.mynah_hip_qwen3_drop(self.h, first, n), "drop")
 
     def set_prefill(self, mode: int) -> None:
         """PREFILL_BATCHED (default) or PREFILL_STEPS for prompt()."""

@@ -172,3 +172,13 @@ def test_element_types():
         list(E.to_e4m3(np.array([16.0, 20.0, 0.0, 2.0 ** -8, 448.0])))
     x = np.array([1.0, -2.5, 1.00390625, 1.01171875, np.inf], np.float32)
     assert list(E.decode(E.encode(x, E.BF16), E.BF16)) == [1.0, -2.5, 1.0, 1.015625, np.inf]
+
+
+# ── the decoder's paths ──────────────────────────────────────────────────────
+
+def test_decoder_without_a_state():
+    t = np.zeros(4, np.uint32)
+    assert M.lib.mynah_hip_qwen3_verify(None, M.ptr(t), None, 4, M.ptr(t), None) == -1
+    assert "verify" in error()
+    assert M.lib.mynah_hip_qwen3_accept(None, M.ptr(t), 4) == -1 and "accept" in error()
+    assert M.lib.mynah_hip_qwen3_drop(None, 0, 0) == -1 and "drop" in error()
