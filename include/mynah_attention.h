@@ -123,8 +123,8 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  * whatever their keys and values hold. mask NULL: node i sees nodes 0 .. i (a chain: several tokens
  * in order, or one). Statistics and sums are held in 32 bits; of 16-bit types
  * the probabilities are rounded to the type for the product with V, the
- * result once. The sums' order depends on the sizes and max_* values alone, so
- * equal calls give equal bits.
+ * result once. The sums' order depends on the sizes, max_* values and lengths
+ * alone, so equal calls give equal bits.
  *   - position p of sequence b is cache row pages[b][p / page_size] * page_size
  *     + p % page_size, or without pages b * seq_slots + p; a row outside
  *     [0, n_slots) (a page id that is no page) is not read and counts as unseen;
@@ -136,7 +136,8 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  *     touched, and a negative n_past counts as 0;
  *   - head_dim 64, 128 or 256; 1 <= n_heads / n_kv_heads <= 64; page_size a
  *     power of two from 16 on; q, out, caches and strides aligned to 16 bytes;
- *     slot_stride below 2^24 bytes; max_kv <= 2^26, and with a mask max_nodes <= 32 * mask_words. */
+ *     slot_stride below 2^24 bytes; max_kv <= 2^26, and with a mask max_nodes <= 32 *
+ *     mask_words and n_rows * mask_words < 2^32. */
 typedef struct {
     int type;                                   /* of q, out and the caches */
     uint32_t n_seqs, n_heads, n_kv_heads, head_dim;

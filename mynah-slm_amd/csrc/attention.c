@@ -222,10 +222,11 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *p, void *stream) {
 /* ── attention of drafted tokens over a cache ────────────────────────────── */
 
 /* What a call launches: kernel `variant` of its type and head size, 16 * nt query
- * rows for each of rw row waves, `waves` waves a workgroup, positions in `splits`
- * runs. */
+ * rows for each of rw row waves, `waves` waves a workgroup, a workgroup for each
+ * key head, group of rows and slot: a sequence's, or with more slots than sequences a
+ * piece of one. */
 typedef struct {
-    uint32_t variant, nt, rw, waves, groups, splits;
+    uint32_t variant, nt, rw, waves, groups, slots;
 } tree_plan;
 
 static int tree_check(const mynah_tree_attention *p) {
@@ -251,6 +252,8 @@ static int tree_check(const mynah_tree_attention *p) {
         return refuse("tree_attention: bad counts (sequences, rows, nodes, positions or slots)");
     if (p->mask != NULL && (p->mask_words == 0 || p->max_nodes > 32ull * p->mask_words))
         return refuse("tree_attention: mask_words too few for max_nodes");
+    if (p->mask != NULL && (uint64_t)p->n_rows * p->mask_words > UINT32_MAX)
+        return refuse("tree_attention: a mask of more than 2^32 words");
     if (p->pages != NULL) {
         if (p->page_size < 16 || (p->page_size & (p->page_size - 1)) != 0)
             return refuse("tree_attention: page_size must be a power of two from 16 on");
@@ -302,17 +305,19 @@ static void tree_make_plan(const mynah_tree_attention *p, uint32_t cus, tree_pla
     /* One workgroup fills a CU's LDS, so at most one for each CU: 264 on 256 CUs
      * took 39 us where 240 take 22. Two or three turns of smaller ones are slower
      * too (16 sequences of 8192 bf16 positions 99, 109 and 121 us). */
-    const uint64_t base = (uint64_t)p->n_seqs * p->n_kv_heads * t->groups;
+    const uint64_t base = (uint64_t)p->n_kv_heads * t->groups;
     const uint32_t turn = t->waves / t->rw * (f32 ? 16u : 32u) * (t->rw > 1 ? 2u : 1u);
-    const uint64_t turns = (p->max_kv + turn - 1) / turn;
+    const uint64_t turns = (uint64_t)p->n_seqs * ((p->max_kv + turn - 1) / turn);
     uint64_t s = cus / base;
     if (s > turns) s = turns;
-    t->splits = s ? (uint32_t)s : 1u;
+    if (s > 256) s = 256;                       /* four sequences a lane share them */
+    t->slots = s > p->n_seqs ? (uint32_t)s : p->n_seqs;
 }
 
 static size_t tree_ws(const mynah_tree_attention *p, const tree_plan *t) {
-    if (t->splits < 2) return 256;
-    return (size_t)t->splits * p->n_rows * p->n_heads * (p->head_dim + 2) * sizeof(float) + 256;
+    if (t->slots == p->n_seqs) return 256;
+    const size_t rows = (size_t)t->slots * p->n_kv_heads * t->groups * 16 * t->nt * t->rw;
+    return rows * (p->head_dim + 2) * sizeof(float) + 2 * (size_t)p->n_seqs * sizeof(int32_t) + 256;
 }
 
 size_t mynah_hip_tree_attention_workspace(const mynah_tree_attention *p) {
@@ -361,10 +366,13 @@ int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
     a.seq_start = p->seq_start;
     a.n_past = p->n_past;
     a.mask = p->mask;
-    const size_t parts = (size_t)t.splits * p->n_rows * p->n_heads;
+    a.wg_rows = 16 * t.nt * t.rw;
+    const uint64_t wgs = (uint64_t)t.slots * p->n_kv_heads * t.groups;
+    const size_t parts = (size_t)wgs * a.wg_rows;
     a.po = (float *)workspace;
     a.pm = a.po + parts * p->head_dim;
     a.pl = a.pm + parts;
+    a.plan = (int32_t *)(a.pl + parts);
     a.n_slots = p->n_slots;
     a.n_seqs = p->n_seqs;
     a.n_heads = p->n_heads;
@@ -377,7 +385,7 @@ int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
     a.mask_words = p->mask_words;
     a.max_nodes = p->max_nodes;
     a.max_kv = p->max_kv;
-    a.splits = t.splits;
+    a.slots = t.slots;
     a.groups = t.groups;
     /* Queries change sign where the scale is negative; no scale counts as a
      * very small one (a score of 0 within 2^-20 for products up to 10^24), so
@@ -387,11 +395,10 @@ int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
     if (p->scale < 0.0f) a.flip = p->type == MYNAH_F32 ? 0x80000000u : 0x80008000u;
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a};
-    const uint64_t wgs = (uint64_t)p->n_seqs * t.splits * p->n_kv_heads * t.groups;
     if (wgs > 0x7fffffffu) return refuse("tree_attention: too many workgroups for one launch");
     if (mynah_launch(d, tree_kernel(p, t.variant), (unsigned)wgs, 1, 64 * t.waves, 0, st, args) != 0)
         return -1;
-    if (t.splits < 2) return 0;
+    if (t.slots == p->n_seqs) return 0;
     const int h = p->head_dim == 64 ? 0 : p->head_dim == 128 ? 1 : 2;
     return mynah_launch3(d, MYNAH_K_TREE_JOIN + 3 * type_index(p->type) + h, p->n_seqs,
                          p->max_nodes, (p->n_heads + 3) / 4, 256, 0, st, args);

@@ -378,9 +378,10 @@ typedef struct {
     const int32_t *pages, *seq_start, *n_past;
     const uint32_t *mask;
     float *pm, *pl, *po;
+    int32_t *plan;
     unsigned long long n_slots;
     uint32_t n_seqs, n_heads, n_kv, group, n_rows, page_log2, max_pages, mask_words;
-    uint32_t max_nodes, max_kv, splits, groups;
+    uint32_t max_nodes, max_kv, slots, groups, wg_rows;
     float scale2;
     uint32_t flip;
 } mynah_tree_args;

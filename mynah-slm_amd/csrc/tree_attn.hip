@@ -16,10 +16,10 @@
 //
 // Bound by memory where a key head has few rows, by the matrix and exponential
 // units where it has many. Measured, MI355X: 16 sequences of 16 nodes over up to
-// 8207 bf16 positions in pages (32 heads, 8 of keys, 128 wide; 288 MB) 99 us, 2.9
-// TB/s; the same with one node each 78 us, 3.7 TB/s; 64 nodes over 130,065 f16
-// positions (533 MB, 136 GFLOP) 198 us; one sequence of 16 nodes over 65,552 60 us,
-// 4.5 TB/s, of one node 51 us, 5.2 TB/s; 24 f32 nodes over 2072 positions 21 us; one
+// 8207 bf16 positions in pages (32 heads, 8 of keys, 128 wide; 288 MB) 96 us, 3.0
+// TB/s; the same with one node each 75 us, 3.8 TB/s; 64 nodes over 130,065 f16
+// positions (533 MB, 136 GFLOP) 206 us; one sequence of 16 nodes over 65,552 61 us,
+// 4.4 TB/s, of one node 53 us, 5.1 TB/s; 24 f32 nodes over 2072 positions 21 us; one
 // f32 token over 513 13 us.
 //
 // SPDX-License-Identifier: MIT
@@ -33,10 +33,11 @@ struct TreeArgs {
     size_t q_stride, out_stride, slot_stride, seq_slots;
     const int32_t *pages, *seq_start, *n_past;
     const uint32_t *mask;
-    float *pm, *pl, *po;            // partials [split][n_rows * n_heads], (x head_dim)
+    float *pm, *pl, *po;            // partials [workgroup][wg_rows], (x head_dim)
+    int32_t *plan;                  // a sequence's first slot and their number
     unsigned long long n_slots;
     uint32_t n_seqs, n_heads, n_kv, group, n_rows, page_log2, max_pages, mask_words;
-    uint32_t max_nodes, max_kv, splits, groups;
+    uint32_t max_nodes, max_kv, slots, groups, wg_rows;
     float scale2;                   // |scale| log2(e), above 0
     uint32_t flip;                  // sign bits of a query's dwords, where scale is below 0
 };
@@ -68,6 +69,93 @@ MYNAH_DEV SeqSpan seq_span(const TreeArgs &a, uint32_t b) {
     const unsigned long long kv = (unsigned long long)s.past + s.nodes;
     s.kv = kv < a.max_kv ? (uint32_t)kv : a.max_kv;
     return s;
+}
+
+// A slot (a workgroup of each key head and group of rows): positions split * per ..
+// of sequence b, `per` at most.
+struct SlotShare {
+    uint32_t b, split, per;
+};
+
+// Several sequences share the slots by their lengths: of 64 sizes of a piece, in
+// turns of the key groups, the smallest that cuts all sequences into no more pieces
+// than there are slots. A lane holds every 64th sequence's turns, and then tries one
+// size; ceil(n * (1 / size)) in floats is the exact number or, where size divides n, at most
+// one more (n < 2^22), and every workgroup finds the same. Sizes run up to
+// total / (slots - n_seqs) + 1, for sum ceil(n / p) <= total / p + n_seqs. False for
+// a slot that is left over. Against as many pieces for every sequence, bf16, 32 heads, 8
+// of keys, 8 nodes: one sequence of 32,768 positions beside 15 of 512 51 us for 209, 4 of
+// 16,000 beside 12 of 1000 76 for 138, 16 of 4000 54 for 52. Exactly equal shares,
+// with slots that end one sequence and begin the next, cost more than they gave: the
+// 16 sequences below 110 us for 96.
+#define TA_MOST_TURNS (1u << 21)    // 2^26 positions in the smallest turn, 32
+MYNAH_DEV bool share_slots(const TreeArgs &a, uint32_t slot, uint32_t turn, bool tell,
+                           SlotShare &out) {
+    const uint32_t lane = threadIdx.x & 63u;
+    float n[4];
+    uint32_t total = 0u;            // at most 255 * 2^21
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t b = 64u * c + lane;
+        uint32_t turns = 0u;
+        if (b < a.n_seqs) {
+            const long long rows = (long long)a.seq_start[b + 1u] - a.seq_start[b];
+            const uint32_t nodes = rows <= 0 ? 0u
+                                 : rows < (long long)a.max_nodes ? (uint32_t)rows : a.max_nodes;
+            const int past = a.n_past[b];
+            const unsigned long long kv = (unsigned long long)(past > 0 ? past : 0) + nodes;
+            const uint32_t k = kv < a.max_kv ? (uint32_t)kv : a.max_kv;
+            turns = nodes ? (k + turn - 1u) / turn : 0u;
+        }
+        n[c] = (float)turns;
+        total += turns;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d /= 2) total += __shfl_xor(total, d, 64);
+    uint32_t least = (total + a.slots - 1u) / a.slots;
+    least = least ? least : 1u;
+    const uint32_t most = total / (a.slots - a.n_seqs) + 1u;
+    uint32_t size = least + (most - least + 61u) / 62u * lane;
+    // A whole sequence a piece is few enough in any case.
+    size = size < TA_MOST_TURNS && lane != 63u ? size : TA_MOST_TURNS;
+    float inv = 1.0f / (float)size, pieces = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t left = a.n_seqs > 64u * c ? a.n_seqs - 64u * c : 0u;
+        for (uint32_t j = 0; j < (left < 64u ? left : 64u); j++)
+            pieces += ceilf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(n[c]), j)) * inv);
+    }
+    const uint32_t pick =
+        (uint32_t)__builtin_ctzll(__ballot(pieces <= (float)a.slots || lane == 63u));
+    inv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inv), pick));
+    out.per = turn * __builtin_amdgcn_readlane(size, pick);
+    uint32_t before = 0u;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t count = (uint32_t)ceilf(n[c] * inv);
+        uint32_t upto = count;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t x = __shfl_up(upto, d, 64);
+            upto += lane >= (uint32_t)d ? x : 0u;
+        }
+        // Sequences that end at or before this slot.
+        const uint32_t at =
+            (uint32_t)__builtin_popcountll(__ballot(before + upto <= slot));
+        if (at < 64u) {
+            const uint32_t mine = __builtin_amdgcn_readlane(count, at);
+            const uint32_t first = before + __builtin_amdgcn_readlane(upto, at) - mine;
+            out.b = 64u * c + at;
+            out.split = slot - first;
+            if (tell && out.split == 0u && threadIdx.x == 0u) {
+                a.plan[2u * out.b] = (int32_t)first;
+                a.plan[2u * out.b + 1u] = (int32_t)mine;
+            }
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
 }
 
 MYNAH_DEV float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -173,9 +261,9 @@ MYNAH_DEV bool cache_row(const TreeArgs &a, uint32_t b, uint32_t p, unsigned lon
 //     barrier a chunk: what comes from the L2 is read by RW waves. (Alone, each wave
 //     with its own rows and keys, 256 rows over 130,001 f16 positions read 4.3 GB
 //     through the L2 at 14-16 TB/s, 278 us.)
-// Grid n_seqs * splits * n_kv * groups (of 16 NT RW query rows), block 64 W.
-// Workgroups go to the 8 XCDs in turn; each XCD takes a run of the order (sequence,
-// split, key head, group), so that groups that share keys share its L2.
+// Grid slots * n_kv * groups (of 16 NT RW query rows), block 64 W. Workgroups go to
+// the 8 XCDs in turn; each XCD takes a run of the order (slot, key head, group), so
+// that groups that share keys share its L2.
 template <class T, int HD, int NT, int RW>
 MYNAH_DEV void tree_attn(const TreeArgs &a) {
     using S = TaShape<T, HD>;
@@ -187,38 +275,63 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
     __shared__ __attribute__((aligned(16))) uint8_t kx[BUF > HALF ? BUF : HALF], vx[BUF];
     __shared__ __attribute__((aligned(16))) uint8_t ky[RW > 1 ? BUF : 16], vy[RW > 1 ? BUF : 16];
     __shared__ float lmax[S::W][16], lsum[S::W][16];
-    __shared__ uint32_t lbad[S::W];
+    __shared__ uint32_t lbad[S::W], keep[8];
+    // Each wave's own: its columns' nodes, and their first words of the mask.
+    __shared__ uint32_t lnode[S::W][16 * NT], lwords[S::W][16 * NT];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lane = threadIdx.x & 63u, lm = lane & 15u, lk = lane >> 4;
     const uint32_t rw = wave % RW, kg = wave / RW;
     uint32_t id = blockIdx.x;
     const uint32_t even = gridDim.x & ~7u;
     if (id < even) id = (id & 7u) * (even >> 3) + (id >> 3);
-    const uint32_t head_id = id / a.groups, part = head_id / a.n_kv, b = part / a.splits;
-    const uint32_t kvh = head_id - part * a.n_kv, split = part - b * a.splits;
+    const uint32_t head_id = id / a.groups, slot = head_id / a.n_kv;
+    const uint32_t kvh = head_id - slot * a.n_kv, part = id - head_id * a.groups;
+    const uint32_t turn = S::CK * KW;              // keys that the groups take at a time
+    SlotShare share = {slot, 0u, ~0u};
+    if (a.slots > a.n_seqs) {                      // uniform
+        if (a.n_seqs == 1u) share = {0u, slot, 0u};
+        else if (!share_slots(a, slot, turn, kvh == 0u && part == 0u, share)) return;
+    }
+    // The compiler does not see that these are the wave's, and walks over lanes else (64
+    // f16 nodes over 130,065 positions 231 us for 209).
+    const uint32_t b = __builtin_amdgcn_readfirstlane(share.b);
+    const uint32_t split = __builtin_amdgcn_readfirstlane(share.split);
     const SeqSpan sq = seq_span(a, b);
     const uint32_t rows = sq.nodes * a.group;
-    const uint32_t wg0 = (id - head_id * a.groups) * (16u * NT * RW);
+    const uint32_t wg0 = part * (16u * NT * RW);
     if (wg0 >= rows) return;                       // uniform
     const uint32_t rr0 = wg0 + 16u * NT * rw;      // the wave's first row
-    const uint32_t turn = S::CK * KW;              // keys that the groups take at a time
-    uint32_t per = (sq.kv + a.splits - 1u) / a.splits;
-    per = (per + turn - 1u) / turn * turn;
-    const uint32_t begin = split * per < sq.kv ? split * per : sq.kv;
+    uint32_t per = __builtin_amdgcn_readfirstlane(share.per);
+    if (per == 0u) {
+        per = (sq.kv + a.slots - 1u) / a.slots;
+        per = (per + turn - 1u) / turn * turn;
+    }
+    const unsigned long long from = (unsigned long long)split * per;
+    const uint32_t begin = from < sq.kv ? (uint32_t)from : sq.kv;
     const uint32_t end = sq.kv - begin < per ? sq.kv : begin + per;
+
+    // What only the end or a mask needs waits in the LDS: in registers it would
+    // spill.
+    if (threadIdx.x == 0u) {
+        keep[0] = id;
+        keep[1] = kvh;
+        keep[2] = wg0;
+        keep[3] = rows;
+        keep[4] = (uint32_t)sq.row0;
+        keep[5] = b;
+        keep[6] = begin;
+    }
 
     // Queries: lane's column of each tile, as operands. Columns that are no query
     // (past the rows) hold zeros, read from row 0.
     uint4 qv[NT][S::KP];
-    uint32_t node[NT];
-    size_t qwords[NT];              // a query's first word of the mask
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const uint32_t rr = rr0 + 16u * n + lm, nd = rr / a.group;
         const long long qrow = sq.row0 + nd;
         const bool live = rr < rows && qrow >= 0 && qrow < (long long)a.n_rows;
-        node[n] = nd;
-        qwords[n] = live ? (size_t)qrow * a.mask_words : 0;
+        lnode[wave][16 * n + lm] = nd;
+        lwords[wave][16 * n + lm] = live ? (uint32_t)qrow * a.mask_words : 0u;
         const char *p = (const char *)a.q + ((live ? (size_t)qrow * a.q_stride : 0) +
                                              (size_t)(kvh * a.group + rr - nd * a.group) * HD) *
                                                 sizeof(T);
@@ -426,7 +539,8 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
                     // a branch here (ROCm 7.2, one f32 kernel).
                     const uint32_t j = p < sq.past ? 0u : p - sq.past;
                     const uint32_t ok =
-                        sees_node(a, qwords[n], node[n], j < sq.nodes ? j : sq.nodes - 1u) |
+                        sees_node(a, lwords[wave][16 * n + lm], lnode[wave][16 * n + lm],
+                                  j < sq.nodes ? j : sq.nodes - 1u) |
                         (uint32_t)(p < sq.past);
                     s[n][t][r] = (ok & (uint32_t)(i < cnv[t])) ? s[n][t][r] : -INFINITY;
                 }
@@ -501,7 +615,11 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
     };
     __builtin_amdgcn_s_waitcnt(0x0f70);                                 // no copy outlives the chunks' place
     if (__any(bad)) bad = true;
-    const size_t heads_all = (size_t)a.n_rows * a.n_heads;
+    __syncthreads();
+    auto kept = [&](int i) { return (uint32_t)__builtin_amdgcn_readfirstlane(keep[i]); };
+    const uint32_t id_ = kept(0), kvh_ = kept(1), wg0_ = kept(2), rows_ = kept(3), b_ = kept(5);
+    const uint32_t begin_ = kept(6);
+    const long long row0_ = (int32_t)kept(4);
 #pragma unroll
     for (int h = 0; h < 2 * NT; h++) {
         const int n = h / 2;
@@ -532,9 +650,9 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
         for (uint32_t i = threadIdx.x; i < 2u * HD * RW; i += 64u * S::W) {
             const uint32_t of = i / (2u * HD), col = i / (HD / 8u) % 16u;
             const uint32_t d = i % (HD / 8u) * 4u + h % 2 * (HD / 2u);
-            const uint32_t rr = wg0 + 16u * (NT * of + n) + col, nd = rr / a.group;
-            const long long orow = sq.row0 + nd;
-            if (rr >= rows || orow < 0 || orow >= (long long)a.n_rows) continue;
+            const uint32_t rr = wg0_ + 16u * (NT * of + n) + col, nd = rr / a.group;
+            const long long orow = row0_ + nd;
+            if (rr >= rows_ || orow < 0 || orow >= (long long)a.n_rows) continue;
             float top = -INFINITY, all = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             uint32_t any_bad = 0u;
 #pragma unroll
@@ -554,24 +672,24 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
                 v[2] = fmaf(f, x.z, v[2]);
                 v[3] = fmaf(f, x.w, v[3]);
             }
-            const uint32_t head = kvh * a.group + rr - nd * a.group;
+            const uint32_t head = kvh_ * a.group + rr - nd * a.group;
             if (any_bad) {
                 // Infinities and NaN of the nodes this row sees: whatever their
                 // share, the sum becomes theirs.
-                for (uint32_t p = sq.past > begin ? sq.past : begin; p < end; p++) {
+                for (uint32_t p = sq.past > begin_ ? sq.past : begin_; p < end; p++) {
                     unsigned long long r;
                     if (!sees_node(a, (size_t)orow * a.mask_words, nd, p - sq.past) ||
-                        !cache_row(a, b, p, r))
+                        !cache_row(a, b_, p, r))
                         continue;
-                    const T *x = (const T *)a.v + r * a.slot_stride + (size_t)kvh * HD + d;
+                    const T *x = (const T *)a.v + r * a.slot_stride + (size_t)kvh_ * HD + d;
                     for (int k = 0; k < 4; k++) {
                         const float y = (float)x[k];
                         if (!(fabsf(y) < INFINITY)) v[k] += y;
                     }
                 }
             }
-            if (a.splits > 1u) {
-                const size_t at = split * heads_all + (size_t)orow * a.n_heads + head;
+            if (a.slots > a.n_seqs) {
+                const size_t at = (size_t)id_ * (16u * NT * RW) + (rr - wg0_);
                 if (d == 0u) {
                     a.pm[at] = top;
                     a.pl[at] = all;
@@ -597,32 +715,39 @@ MYNAH_DEV void tree_join(const TreeArgs &a) {
     const SeqSpan sq = seq_span(a, b);
     const long long row = sq.row0 + nd;
     if (nd >= sq.nodes || row < 0 || row >= (long long)a.n_rows || head >= a.n_heads) return;
-    const size_t heads_all = (size_t)a.n_rows * a.n_heads;
-    const size_t at = (size_t)row * a.n_heads + head;
+    // A split's place in the partials, and how far the next split's is.
+    const uint32_t kvh = head / a.group, rr = nd * a.group + head - kvh * a.group;
+    const uint32_t part = rr / a.wg_rows;
+    const bool one = a.n_seqs == 1u;
+    const uint32_t first = one ? 0u : (uint32_t)scalar_i32(a.plan, 2u * b);
+    const uint32_t splits = one ? a.slots : (uint32_t)scalar_i32(a.plan, 2u * b + 1u);
+    const size_t step = (size_t)a.n_kv * a.groups * a.wg_rows;
+    const size_t at = first * step + ((size_t)kvh * a.groups + part) * a.wg_rows +
+                      (rr - part * a.wg_rows);
     // A split's maximum and sum to each lane, 64 of them at a time.
     float top = -INFINITY;
-    for (uint32_t s = lane; s < a.splits; s += 64u) top = fmaxf(top, a.pm[s * heads_all + at]);
+    for (uint32_t s = lane; s < splits; s += 64u) top = fmaxf(top, a.pm[s * step + at]);
     top = wave_max_dpp(top);
     const float base = top == -INFINITY ? 0.0f : top;
     float all = 0.0f, v[E];
 #pragma unroll
     for (int i = 0; i < E; i++) v[i] = 0.0f;
-    for (uint32_t s0 = 0u; s0 < a.splits; s0 += 64u) {
-        const uint32_t n = a.splits - s0 < 64u ? a.splits - s0 : 64u;
-        const size_t from = (s0 + lane) * heads_all + at;
+    for (uint32_t s0 = 0u; s0 < splits; s0 += 64u) {
+        const uint32_t n = splits - s0 < 64u ? splits - s0 : 64u;
+        const size_t from = (s0 + lane) * step + at;
         const float w = lane < n ? exp2_hw(a.pm[from] - base) : 0.0f;
         all += lane < n ? w * a.pl[from] : 0.0f;
         auto weight = [&](uint32_t s) {
             return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
         };
-        const float *p = a.po + (s0 * heads_all + at) * HD + E * lane;
+        const float *p = a.po + (s0 * step + at) * HD + E * lane;
         uint32_t s = 0u;
         for (; s + 8u <= n; s += 8u) {             // eight loads under way
             float x[8][E];
 #pragma unroll
             for (int j = 0; j < 8; j++)
 #pragma unroll
-                for (int i = 0; i < E; i++) x[j][i] = p[(s + j) * heads_all * HD + i];
+                for (int i = 0; i < E; i++) x[j][i] = p[(s + j) * step * HD + i];
 #pragma unroll
             for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -630,7 +755,7 @@ MYNAH_DEV void tree_join(const TreeArgs &a) {
         }
         for (; s < n; s++)
 #pragma unroll
-            for (int i = 0; i < E; i++) v[i] = fmaf(weight(s), p[s * heads_all * HD + i], v[i]);
+            for (int i = 0; i < E; i++) v[i] = fmaf(weight(s), p[s * step * HD + i], v[i]);
     }
     all = wave_sum(all);
     T *y = (T *)a.out + (size_t)row * a.out_stride + (size_t)head * HD + E * lane;

@@ -122,7 +122,7 @@ TREE = dict(type=30, n_seqs=2, n_heads=8, n_kv_heads=2, head_dim=128, q=P, q_str
     {"type": 8}, {"q": None}, {"out": None}, {"k_cache": None}, {"v_cache": None},
     {"seq_start": None}, {"n_past": None}, {"head_dim": 96}, {"head_dim": 0}, {"n_heads": 0},
     {"n_kv_heads": 0}, {"n_heads": 7}, {"n_heads": 130}, {"n_seqs": 0}, {"n_rows": 0},
-    {"max_nodes": 0}, {"max_nodes": 65536, "mask": None}, {"max_kv": 0}, {"max_kv": (1 << 26) + 1},
+    {"n_rows": 1 << 31, "mask_words": 2}, {"max_nodes": 0}, {"max_nodes": 65536, "mask": None}, {"max_kv": 0}, {"max_kv": (1 << 26) + 1},
     {"n_slots": 0}, {"mask_words": 0}, {"max_nodes": 33}, {"page_size": 8}, {"page_size": 24},
     {"page_size": 0}, {"max_kv": 33}, {"pages": None, "seq_slots": 1 << 40}, {"q_stride": 1000},
     {"out_stride": 512}, {"slot_stride": 128}, {"slot_stride": (1 << 24) + 8}, {"q": P + 8},

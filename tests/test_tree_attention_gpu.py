@@ -174,6 +174,21 @@ def test_more_splits_than_lanes(M, t, hd):
     c.check(c.call())
 
 
+RAGGED = [[(9000, 4)] + [(20, 2)] * 15, [(0, 0)] * 3 + [(5000, 3), (0, 0), (1, 1)], [(0, 0)] * 4,
+          [(40 * i % 1201, i % 4) for i in range(70)], [(i % 3, i % 2) for i in range(200)]]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("lens", RAGGED, ids=lambda v: f"{len(v)}-{max(v)[0]}")
+def test_ragged_batches(M, t, lens):
+    # Sequences of very different lengths are cut into pieces by theirs.
+    print("[case] tree ragged", t, len(lens), flush=True)
+    c = Tree(M, lens, 2, 1, 64, t, page=16, seed=7, extra_rows=1)
+    raw = c.call()
+    c.check(raw)
+    assert np.array_equal(raw, c.call())
+
+
 def test_one_workspace_byte_short(M):
     c = Tree(M, [(900, 2)], 4, 1, 128, E.F32)
     a = c.args()
