@@ -303,8 +303,9 @@ static void tree_make_plan(const mynah_tree_attention *p, uint32_t cus, tree_pla
     }
     t->groups = (uint32_t)((tiles + t->nt * t->rw - 1) / (t->nt * t->rw));
     /* One workgroup fills a CU's LDS, so at most one for each CU: 264 on 256 CUs
-     * took 39 us where 240 take 22. Two or three turns of smaller ones are slower
-     * too (16 sequences of 8192 bf16 positions 99, 109 and 121 us). */
+     * took 39 us where 240 take 22. Two or three workgroups a CU, one after the
+     * other, are slower too (16 sequences of up to 8207 bf16 positions cut alike 99,
+     * 109 and 121 us). */
     const uint64_t base = (uint64_t)p->n_kv_heads * t->groups;
     const uint32_t turn = t->waves / t->rw * (f32 ? 16u : 32u) * (t->rw > 1 ? 2u : 1u);
     const uint64_t turns = (uint64_t)p->n_seqs * ((p->max_kv + turn - 1) / turn);

@@ -20,7 +20,7 @@ typedef float fp8_v4f __attribute__((ext_vector_type(4)));
 // (448 * (1 / amax))), each operation rounded to f32, e4m3 to nearest, ties to
 // even. 16 lanes a block, 8 values a lane; a NaN
 // stays NaN, an infinity makes its block's scale infinite (and its product
-// NaN). What bounds it: HBM (or the launch, for few tokens).
+// NaN). What bounds it: HBM, or the launch for few tokens (37 x 2560 bf16: 2.4 us).
 template <class T>
 MYNAH_DEV void fp8_quantize(const T *x, size_t x_stride, uint32_t cols, uint32_t nb,
                             unsigned long long blocks, uint8_t *xq, float *xs) {
@@ -74,7 +74,9 @@ FP8_QUANT_KERNEL(bf16, __bf16)
 // (l / 16) of a block, the same places of both operands, so each load of a wave
 // takes 64 contiguous bytes of 16 rows, straight into the operand's registers;
 // its results are token l % 16, rows 4 (l / 16) + 0..3.
-// What bounds it: HBM, the weights being read once.
+// What bounds it: HBM, the weights being read once (9728 x 2560, one token, f32 out:
+// 6.4 us a call, 3.9 TB/s), and for more tokens the loads of few workgroups (4096 x
+// 2560, 37 tokens, bf16 out: 256 of them, 8.0 us).
 struct Fp8Chunk { uint4 lo, hi; };
 MYNAH_DEV Fp8Chunk fp8_chunk(const uint8_t *row, uint32_t k) {
     return Fp8Chunk{*(const uint4 *)(row + k), *(const uint4 *)(row + k + 64u)};

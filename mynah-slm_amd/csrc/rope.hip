@@ -57,7 +57,11 @@ MYNAH_DEV void turn(double p, double f, float mscale, float &c, float &s) {
 // values from 8 l on. A slot of lanes keeps one token's cos and sin over the
 // heads g, g + groups, ... of its group.
 // What bounds it: HBM on long inputs, the launch and one chain of dependent
-// loads (position, frequency, row) on single tokens.
+// loads (position, frequency, row) on single tokens. Measured, MI355X: 8192 tokens of
+// 32 heads of 128 bf16 (134 MB) 41 us, 3.3 TB/s (a copy of the size 26; 27 where
+// the last-level cache holds them), 2047 tokens of 40 f32 heads with norms to bf16
+// rows 18.2 us, one token 4 us. One head a lane took 46 us (an angle for each), rows
+// loaded two or four ahead of their use 52.
 template <class TI, class TO, bool HALF, bool VEC>
 MYNAH_DEV void rope_rows(const RopeArgs &a) {
     const uint32_t ll = a.lanes_log2, l = threadIdx.x & ((1u << ll) - 1u);

@@ -15,9 +15,9 @@
 // end, workgroups in a second launch.
 //
 // Bound by memory where a key head has few rows, by the matrix and exponential
-// units where it has many. Measured, MI355X: 16 sequences of 16 nodes over up to
-// 8207 bf16 positions in pages (32 heads, 8 of keys, 128 wide; 288 MB) 96 us, 3.0
-// TB/s; the same with one node each 75 us, 3.8 TB/s; 64 nodes over 130,065 f16
+// units where it has many. Measured, MI355X: 16 sequences of up to 16 nodes and
+// 8207 bf16 positions in pages (32 heads, 8 of keys, 128 wide; 85,413 positions in all,
+// 350 MB) 96 us, 3.6 TB/s; the same with one node each 75 us, 4.7 TB/s; 64 nodes over 130,065 f16
 // positions (533 MB, 136 GFLOP) 206 us; one sequence of 16 nodes over 65,552 61 us,
 // 4.4 TB/s, of one node 53 us, 5.1 TB/s; 24 f32 nodes over 2072 positions 21 us; one
 // f32 token over 513 13 us.
