@@ -231,6 +231,22 @@ def test_drop_at_the_end_is_an_undo(M, model):
     dec.drop(0, 0)
 
 
+@pytest.mark.parametrize("mode", ["ATTN_EXACT", "ATTN_SPLIT"])
+@pytest.mark.parametrize("late,early", [(100, 50), (600, 3)])
+def test_steps_captured_late_run_early(M, model, mode, late, early):
+    # A step's graph that was captured further on runs again after a drop.
+    a, b = decoder(M, model, late, late + 20), decoder(M, model, early, late + 20)
+    for dec in (a, b):
+        dec.set_attention(getattr(M, mode))
+    a.generate(3, 9)
+    a.verify([1, 2, 3])
+    a.drop(early, a.n_past - early)
+    k, v = O.kv_prefill(O.substream, SHAPE, 0, early)
+    a.set_kv(k, v, early)
+    for t in (5, 6):
+        assert np.array_equal(a.forward(t).view(np.uint32), b.forward(t).view(np.uint32))
+
+
 def test_drop_of_more_rows_than_move_at_a_time(M, model):
     past, n = 9001, 2
     dec = decoder(M, model, past, 9010)
