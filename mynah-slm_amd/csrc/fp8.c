@@ -75,14 +75,26 @@ static const fp8_tile fp8_tiles[5] = {
     {128, 128, 8, 1, {0.65f, 1.09f}, {0.65f, 1.10f}},
     {256, 256, 8, 1, {1.82f, 0.0f}, {2.00f, 0.0f}}};
 
+/* Microseconds of the streaming kernel for 17 to 64 tokens, launch and all: rounds
+ * of 16 weight rows a CU, a step longer with every token. Up to 16 tokens it is
+ * taken in any case. Measured against the tiles, bf16
+ * out: 1024 x 2560, 17 tokens 5.1 for 8.5 us, 64 tokens 8.9 for 8.7; 4096 x 2560, 48
+ * tokens 8.1 for 8.8, 64 tokens 9.3 for 8.8; 9728 x 2560, 16 tokens 9.5 for 8.7, 17
+ * tokens 10.8 for 8.8, 64 tokens 22.4 for 9.0; 2560 x 9728, 48 tokens 23.4 for 24.7, 64
+ * tokens 27.3 for 24.8. */
+static double fp8_few_us(size_t rows, size_t tokens, size_t cols, uint32_t cus) {
+    const double rounds = (double)(((rows + 15) / 16 + cus - 1) / cus);
+    return 2.4 + rounds * (double)((cols + BLOCK - 1) / BLOCK) * (0.085 + 0.0038 * (double)tokens);
+}
+
 /* The tile of least estimated time for a product, or NULL for the streaming
  * kernel: whole rounds of resident workgroups, then a last one. Four steps stand
- * for the start and the end of a workgroup. The tiles address their rows in 32
- * bits. MYNAH_FP8_TILE=0..4 forces one. */
+ * for the start and the end of a workgroup, 1.5 us for the launch. The tiles address
+ * their rows in 32 bits. MYNAH_FP8_TILE=0..4 forces one. */
 static const fp8_tile *fp8_plan(int type, size_t rows, size_t tokens, size_t cols,
                                 uint32_t cus) {
     const int f32 = type == MYNAH_F32, most = f32 ? 3 : 4;
-    if (tokens <= 64 || cols > (size_t)1 << 23) return NULL;
+    if (tokens <= 16 || cols > (size_t)1 << 23) return NULL;
     const char *env = getenv("MYNAH_FP8_TILE");
     if (env != NULL && env[0] >= '0' && env[0] <= '0' + most && env[1] == '\0')
         return &fp8_tiles[env[0] - '0'];
@@ -101,6 +113,7 @@ static const fp8_tile *fp8_plan(int type, size_t rows, size_t tokens, size_t col
             best_us = us;
         }
     }
+    if (tokens <= 64 && fp8_few_us(rows, tokens, cols, cus) <= best_us + 1.5) return NULL;
     return best;
 }
 

@@ -112,6 +112,7 @@ SHAPES = [  # rows, cols, tokens
     (1, 16, 1), (16, 128, 1), (130, 256, 1), (100, 144, 2), (257, 640, 5), (64, 2560, 16),
     (48, 1040, 17), (300, 384, 32), (129, 1168, 33), (1024, 512, 64), (200, 256, 65),
     (384, 128, 130), (513, 912, 127), (256, 1024, 300), (1000, 2048, 257), (640, 272, 1000),
+    (9000, 272, 17), (9000, 144, 40), (4128, 1040, 64), (8208, 400, 33),   # few, in tiles
 ]
 
 
