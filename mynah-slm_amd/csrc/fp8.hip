@@ -278,15 +278,18 @@ MYNAH_DEV void fp8_tile(const uint8_t *w, const float *ws, const uint8_t *xq, co
     auto copy = [&](uint32_t b, uint8_t *p) {
         const uint32_t off = b * FP8_B + 16u * chunk < cols ? 0u : NONE;
         const uint32_t soff = b < nb ? 0u : NONE;
+        // The range check compares an offset with the buffer's size less the block's
+        // place, which past the last block would be below zero.
+        const uint32_t place = b < nb ? b : 0u;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rxs, (fp8_lds_void *)(p + P::XS + 256u * wave),
-                                                 4, xat | soff, 4u * b, 0, 0);
+                                                 4, xat | soff, 4u * place, 0, 0);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rws, (fp8_lds_void *)(p + P::WS + 256u * wave),
-                                                 4, wat | soff, 4u * b, 0, 0);
+                                                 4, wat | soff, 4u * place, 0, 0);
 #pragma unroll
         for (int i = 0; i < P::COPIES; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 i < WC ? rw : rx, (fp8_lds_void *)(p + 1024u * (P::NW * i + wave)), 16,
-                at[i] | off, FP8_B * b, 0, 0);
+                at[i] | off, FP8_B * place, 0, 0);
     };
     const uint32_t a0 = (r0 + lm) * FP8_B + 16u * (lk ^ (lm & 7u));
     const uint32_t b0 = (P::ROWS + t0 + lm) * FP8_B + 16u * (lk ^ (lm & 7u));
