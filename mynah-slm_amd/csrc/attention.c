@@ -7,6 +7,7 @@
 #include "kernels_hip.h"
 #include "runtime_internal.h"
 
+#include <float.h>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -391,8 +392,9 @@ int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
     /* Queries change sign where the scale is negative; no scale counts as a
      * very small one (a score of 0 within 2^-20 for products up to 10^24), so
      * that -inf stays what it is. */
-    a.scale2 = fabsf(p->scale) * 1.44269504088896341f;
+    a.scale2 = fminf(fabsf(p->scale) * 1.44269504088896341f, FLT_MAX);
     if (a.scale2 < 1e-30f) a.scale2 = 1e-30f;
+    a.lag = 8.0f / a.scale2;
     if (p->scale < 0.0f) a.flip = p->type == MYNAH_F32 ? 0x80000000u : 0x80008000u;
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a};

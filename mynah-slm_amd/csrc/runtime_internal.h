@@ -382,7 +382,7 @@ typedef struct {
     unsigned long long n_slots;
     uint32_t n_seqs, n_heads, n_kv, group, n_rows, page_log2, max_pages, mask_words;
     uint32_t max_nodes, max_kv, slots, groups, wg_rows;
-    float scale2;
+    float scale2, lag;
     uint32_t flip;
 } mynah_tree_args;
 

@@ -38,7 +38,8 @@ struct TreeArgs {
     unsigned long long n_slots;
     uint32_t n_seqs, n_heads, n_kv, group, n_rows, page_log2, max_pages, mask_words;
     uint32_t max_nodes, max_kv, slots, groups, wg_rows;
-    float scale2;                   // |scale| log2(e), above 0
+    float scale2;                   // |scale| log2(e), above 0 and finite
+    float lag;                      // growth of a score without a new reference
     uint32_t flip;                  // sign bits of a query's dwords, where scale is below 0
 };
 
@@ -247,11 +248,12 @@ MYNAH_DEV bool cache_row(const TreeArgs &a, uint32_t b, uint32_t p, unsigned lon
     return r < a.n_slots;
 }
 
-// Growth of a column's scores, in powers of two, that its reference for the
-// exponentials is left behind by: sums and 16-bit probabilities hold 2^8 times
-// their size, and most chunks then rescale nothing and compare only within
-// their lanes.
-#define TA_LAG 8.0f
+// A column's reference for the exponentials is left behind by scores that grow up to
+// a.lag (2^8 in the probabilities): sums and 16-bit probabilities hold 2^8 times their
+// size, and most chunks then rescale nothing and compare only within their lanes.
+// References are scores as the products gave them, so that the difference to one is
+// exact next to it and only then scaled: a scaled reference's rounding alone is
+// above a power of two from scores of 2^25 on.
 
 // A workgroup's W waves are RW row waves, each with 16 NT query rows of its own, for
 // each of W / RW key groups, which take chunks of keys in turn.
@@ -474,10 +476,9 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
             float top = s[n][0][0];
 #pragma unroll
             for (int j = 1; j < 4 * S::TILES; j++) top = fmaxf(top, s[n][j / 4][j % 4]);
-            top *= a.scale2;
-            if (__any(top > m[n] + TA_LAG)) {
+            if (__any(top - m[n] > a.lag)) {
                 top = fmaxf(m[n], lane_max4(top));
-                const float f = exp2_hw(m[n] - (top == -INFINITY ? 0.0f : top));
+                const float f = exp2_hw((m[n] - (top == -INFINITY ? 0.0f : top)) * a.scale2);
                 l[n] *= f;
 #pragma unroll
                 for (int e = 0; e < S::VE; e++) o[n][e] *= f;
@@ -488,7 +489,7 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
             if constexpr (S::F32) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float x = exp2_hw(fmaf(s[n][0][r], a.scale2, -base));
+                    const float x = exp2_hw((s[n][0][r] - base) * a.scale2);
                     l[n] += x;
                     p[r] = __float_as_uint(x);
                 }
@@ -496,7 +497,7 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
                 T h[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float x = exp2_hw(fmaf(s[n][j / 4][j % 4], a.scale2, -base));
+                    const float x = exp2_hw((s[n][j / 4][j % 4] - base) * a.scale2);
                     l[n] += x;
                     h[j] = (T)x;
                 }
@@ -664,7 +665,7 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
 #pragma unroll
             for (int k = 0; k < KW; k++) {
                 const uint32_t w = RW * k + of;
-                const float f = exp2_hw(lmax[w][col] - base);
+                const float f = exp2_hw((lmax[w][col] - base) * a.scale2);
                 const float4 x = *(const float4 *)place(w, col, d);
                 all = fmaf(f, lsum[w][col], all);
                 v[0] = fmaf(f, x.x, v[0]);
@@ -735,7 +736,7 @@ MYNAH_DEV void tree_join(const TreeArgs &a) {
     for (uint32_t s0 = 0u; s0 < splits; s0 += 64u) {
         const uint32_t n = splits - s0 < 64u ? splits - s0 : 64u;
         const size_t from = (s0 + lane) * step + at;
-        const float w = lane < n ? exp2_hw(a.pm[from] - base) : 0.0f;
+        const float w = lane < n ? exp2_hw((a.pm[from] - base) * a.scale2) : 0.0f;
         all += lane < n ? w * a.pl[from] : 0.0f;
         auto weight = [&](uint32_t s) {
             return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
