@@ -122,9 +122,10 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  * nothing, or scores of -inf only, is 0. Unseen positions have no effect,
  * whatever their keys and values hold. mask NULL: node i sees nodes 0 .. i (a chain: several tokens
  * in order, or one). Statistics and sums are held in 32 bits; of 16-bit types
- * the probabilities are rounded to the type for the product with V, the
- * result once. The sums' order depends on the sizes, max_* values and lengths
- * alone, so equal calls give equal bits.
+ * the probabilities are rounded to the type for the product with V (f16: of n
+ * positions, those below 2^-25 of the row's largest are off by n 2^-36 of it
+ * together at most), the result once. The sums' order depends on the sizes,
+ * max_* values and lengths alone, so equal calls give equal bits.
  *   - position p of sequence b is cache row pages[b][p / page_size] * page_size
  *     + p % page_size, or without pages b * seq_slots + p; a row outside
  *     [0, n_slots) (a page id that is no page) is not read and counts as unseen;

@@ -394,7 +394,7 @@ int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
      * that -inf stays what it is. */
     a.scale2 = fminf(fabsf(p->scale) * 1.44269504088896341f, FLT_MAX);
     if (a.scale2 < 1e-30f) a.scale2 = 1e-30f;
-    a.lag = 8.0f / a.scale2;
+    a.lag = (p->type == MYNAH_F16 ? 4.0f : 8.0f) / a.scale2;   /* 2^11 2^4 fits an f16 */
     if (p->scale < 0.0f) a.flip = p->type == MYNAH_F32 ? 0x80000000u : 0x80008000u;
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a};

@@ -165,6 +165,7 @@ MYNAH_DEV float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 template <class T, int HD>
 struct TaShape {
     static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr float UP = __is_same(T, _Float16) ? 11.0f : 0.0f; // see a.lag below
     static constexpr int TILES = F32 ? 1 : 2;         // 16-key tiles of a chunk
     static constexpr int CK = 16 * TILES;             // keys of a chunk
     static constexpr int KP = F32 ? HD / 16 : HD / 32; // 16-byte pieces of a lane's key
@@ -249,8 +250,14 @@ MYNAH_DEV bool cache_row(const TreeArgs &a, uint32_t b, uint32_t p, unsigned lon
 }
 
 // A column's reference for the exponentials is left behind by scores that grow up to
-// a.lag (2^8 in the probabilities): sums and 16-bit probabilities hold 2^8 times their
-// size, and most chunks then rescale nothing and compare only within their lanes.
+// a.lag (2^8 in the probabilities, of f16 2^4): sums and 16-bit probabilities hold that
+// many times their size, and most chunks then rescale nothing and compare only within
+// their lanes. f16 probabilities are 2^11 times theirs, for below 2^-14 the type keeps
+// fewer bits and below 2^-25 nothing: with the largest at 2^11 or above, n of them are off
+// by n 2^-36 of it at most, a half step of the result at 2^25 positions. (Unscaled,
+// one position 17.4 nats above 130,000 others lost 0.4 % of the result.) The sums
+// carry the factor too, so it leaves with the division. 64 f16 nodes over 130,065
+// positions, lag and factor 2^8 and 1: 199 us; 2^8, 2^7: 201; 2^4, 2^11: 203; 2^2, 2^13: 208.
 // References are scores as the products gave them, so that the difference to one is
 // exact next to it and only then scaled: a scaled reference's rounding alone is
 // above a power of two from scores of 2^25 on.
@@ -497,7 +504,7 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
                 T h[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float x = exp2_hw((s[n][j / 4][j % 4] - base) * a.scale2);
+                    const float x = exp2_hw(fmaf(s[n][j / 4][j % 4] - base, a.scale2, S::UP));
                     l[n] += x;
                     h[j] = (T)x;
                 }

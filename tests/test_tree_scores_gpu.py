@@ -52,3 +52,35 @@ def test_scores_far_apart(M, t, scale, lens):
 def test_negative_scale(M, t, hd):
     c = Tree(M, [(333, 9), (20, 2)], 6, 2, hd, t, seed=hd, scale=-hd ** -0.5)
     c.check(c.call())
+
+
+@pytest.mark.parametrize("below", [12.0, 15.0, 17.4, 20.0])
+@pytest.mark.parametrize("t", TYPES)
+def test_much_weight_in_small_probabilities(M, t, below):
+    """One position `below` nats above 130,000 others, and values of one sign: each
+    other's probability is small, their sum is not. The bound is that of
+    tree_lib.Tree.expected but for two terms. One key head's positions go to 128
+    workgroups at least, so that no sum is a chain of more than n / 128 additions and
+    those that join 512 waves' and workgroups': n / 128 + 512 in place of n. And an f16
+    probability below the type's smallest normal number is off by up to 2^-25
+    where the row's largest is at least 2^11: n 2^-36 of it at most."""
+    print("[case] small probabilities", t, below, flush=True)
+    hd, n = 64, 130_003
+    c = Tree(M, [(n - 3, 3)], 2, 1, hd, t, mask="chain", seed=5)
+    q = np.zeros(c.q.shape)
+    q[:, ::hd] = 8.0
+    k = 0.01 * c.rng.standard_normal(c.k.shape)
+    k[:, 0] = 0.0
+    k[7, 0] = below                                      # 8 below * 64^-0.5
+    c.q, c.k = E.encode(q, t), E.encode(k, t)
+    c.v = E.encode(1.0 + 0.25 * c.rng.random(c.v.shape), t)
+    raw = c.call()
+    assert c.ws.nbytes > 128 * 16 * (hd + 2) * 4
+    want = c.expected()[0]
+    got = E.decode(raw, t).reshape(want.shape)
+    dm = (hd + 4) * U * below
+    tol = want * (2 * dm + (6 + n / 128 + 512) * U + (0 if t == E.F32 else E.HALF[t]))
+    tol += E.rounded(want, t) + (n * 2.0 ** -36 * 1.25 if t == E.F16 else 0)
+    off = np.abs(got - want) / tol
+    print(f"largest error {float(off.max()):.2f} of its bound", flush=True)
+    assert off.max() <= 1
