@@ -58,30 +58,27 @@ int mynah_hip_fp8_quantize_dev(int type, const void *x, size_t x_stride, size_t 
                         256, 0, mynah_stream_or_default(d, stream), args);
 }
 
-/* The tiled kernels, in the kernel ids' order (the largest has no f32 form): how
- * many workgroups a CU holds, and the microseconds of a step (a block of 128
- * columns) with one a CU and with all of them, for 16-bit and for f32 outputs,
- * measured on MI355X as the slope from 10 to 40 blocks at 256 workgroups and at
- * 2,048. Two of the 4-wave 128 x 128 tile share a CU (1.17 us for both); alone on
- * it the 8-wave one is the faster (0.65 against 0.78). */
+/* The tiled kernels, in the kernel ids' order: how many workgroups a CU holds, and
+ * the microseconds of a step (a block of 128 columns) with one a CU and with all of
+ * them, measured on MI355X as the slope from 10 to 40 blocks at 256 workgroups and at
+ * 2,048 (bf16 outputs; f32 ones within 3 %). Two of the 4-wave 128 x 128 tile share a
+ * CU (1.86 us for both); alone on it the 8-wave one is the faster (0.97 against 1.05
+ * where 128 CUs have one). */
 typedef struct {
     uint32_t rows, toks, waves, per_cu;
-    float one[2], all[2];
+    float one, all;
 } fp8_tile;
-static const fp8_tile fp8_tiles[5] = {
-    {64, 64, 4, 2, {0.29f, 0.42f}, {0.45f, 0.67f}},
-    {64, 128, 4, 2, {0.48f, 0.67f}, {0.82f, 1.15f}},
-    {128, 128, 4, 2, {0.78f, 1.06f}, {1.17f, 1.85f}},
-    {128, 128, 8, 1, {0.65f, 1.09f}, {0.65f, 1.10f}},
-    {256, 256, 8, 1, {1.82f, 0.0f}, {2.00f, 0.0f}}};
+static const fp8_tile fp8_tiles[4] = {{64, 64, 4, 2, 0.43f, 0.69f},
+                                      {64, 128, 4, 2, 0.66f, 1.14f},
+                                      {128, 128, 4, 2, 1.06f, 1.86f},
+                                      {128, 128, 8, 1, 1.05f, 1.05f}};
 
 /* Microseconds of the streaming kernel for 17 to 64 tokens, launch and all: rounds
  * of 16 weight rows a CU, a step longer with every token. Up to 16 tokens it is
- * taken in any case. Measured against the tiles, bf16
- * out: 1024 x 2560, 17 tokens 5.1 for 8.5 us, 64 tokens 8.9 for 8.7; 4096 x 2560, 48
- * tokens 8.1 for 8.8, 64 tokens 9.3 for 8.8; 9728 x 2560, 16 tokens 9.5 for 8.7, 17
- * tokens 10.8 for 8.8, 64 tokens 22.4 for 9.0; 2560 x 9728, 48 tokens 23.4 for 24.7, 64
- * tokens 27.3 for 24.8. */
+ * taken in any case. Measured against the fastest tile, bf16 out: 1024 x 2560, 17
+ * tokens 4.9 for 11.2 us, 64 tokens 8.9 for 11.3; 4096 x 2560, 64 tokens 9.3 for 11.5;
+ * 9728 x 2560, 16 tokens 9.5, 17 tokens 10.9 for 11.5, 24 tokens 12.4 for 11.6, 64 tokens
+ * 22.3 for 11.8; 2560 x 9728, 64 tokens 27.3 for 34.6. */
 static double fp8_few_us(size_t rows, size_t tokens, size_t cols, uint32_t cus) {
     const double rounds = (double)(((rows + 15) / 16 + cus - 1) / cus);
     return 2.4 + rounds * (double)((cols + BLOCK - 1) / BLOCK) * (0.085 + 0.0038 * (double)tokens);
@@ -90,23 +87,21 @@ static double fp8_few_us(size_t rows, size_t tokens, size_t cols, uint32_t cus) 
 /* The tile of least estimated time for a product, or NULL for the streaming
  * kernel: whole rounds of resident workgroups, then a last one. Four steps stand
  * for the start and the end of a workgroup, 1.5 us for the launch. The tiles address
- * their rows in 32 bits. MYNAH_FP8_TILE=0..4 forces one. */
-static const fp8_tile *fp8_plan(int type, size_t rows, size_t tokens, size_t cols,
-                                uint32_t cus) {
-    const int f32 = type == MYNAH_F32, most = f32 ? 3 : 4;
+ * their rows in 32 bits. MYNAH_FP8_TILE=0..3 forces one. */
+static const fp8_tile *fp8_plan(size_t rows, size_t tokens, size_t cols, uint32_t cus) {
     if (tokens <= 16 || cols > (size_t)1 << 23) return NULL;
     const char *env = getenv("MYNAH_FP8_TILE");
-    if (env != NULL && env[0] >= '0' && env[0] <= '0' + most && env[1] == '\0')
+    if (env != NULL && env[0] >= '0' && env[0] <= '3' && env[1] == '\0')
         return &fp8_tiles[env[0] - '0'];
     const fp8_tile *best = NULL;
     double best_us = 0.0;
-    for (int i = 0; i <= most; i++) {
+    for (int i = 0; i < 4; i++) {
         const fp8_tile *t = &fp8_tiles[i];
         const uint64_t wgs = (uint64_t)((rows + t->rows - 1) / t->rows) *
                              (uint64_t)((tokens + t->toks - 1) / t->toks);
         const uint64_t slots = (uint64_t)cus * t->per_cu, left = wgs % slots;
-        double us = (double)(wgs / slots) * t->all[f32];
-        if (left) us += left <= cus ? t->one[f32] : t->all[f32];
+        double us = (double)(wgs / slots) * t->all;
+        if (left) us += left <= cus ? t->one : t->all;
         us *= (double)((cols + BLOCK - 1) / BLOCK + 4);
         if (best == NULL || us < best_us) {
             best = t;
@@ -141,15 +136,14 @@ int mynah_hip_fp8_matmat_dev(const uint8_t *w, const float *ws, size_t rows, siz
              nb = (uint32_t)((cols + BLOCK - 1) / BLOCK);
     hipStream_t st = mynah_stream_or_default(d, stream);
     const int t = type_index(type);
-    const fp8_tile *tl = fp8_plan(type, rows, tokens, cols, (uint32_t)d->cus);
+    const fp8_tile *tl = fp8_plan(rows, tokens, cols, (uint32_t)d->cus);
     if (tl != NULL) {
         uint32_t tr = (uint32_t)((rows + tl->rows - 1) / tl->rows);
         const uint64_t wgs = (uint64_t)tr * ((tokens + tl->toks - 1) / tl->toks);
         if (wgs <= 0x7fffffffu) {
             void *args[] = {&w, &ws, &xq, &xs, &y, &r32, &c32, &t32, &nb, &tr};
-            return mynah_launch(d, MYNAH_K_FP8_TILE + 3 * (int)(tl - fp8_tiles) + t -
-                                (tl == &fp8_tiles[4]), (unsigned)wgs,
-                                1, 64 * tl->waves, 0, st, args);
+            return mynah_launch(d, MYNAH_K_FP8_TILE + 3 * (int)(tl - fp8_tiles) + t, (unsigned)wgs, 1,
+                                64 * tl->waves, 0, st, args);
         }
     }
     void *args[] = {&w, &ws, &xq, &xs, &y, &r32, &c32, &t32, &nb};

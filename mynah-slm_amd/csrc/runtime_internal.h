@@ -154,8 +154,6 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_FP8_128X128W_F32, "mynah_fp8_128x128w_f32") \
     X(MYNAH_K_FP8_128X128W_F16, "mynah_fp8_128x128w_f16") \
     X(MYNAH_K_FP8_128X128W_BF16, "mynah_fp8_128x128w_bf16") \
-    X(MYNAH_K_FP8_256X256_F16, "mynah_fp8_256x256_f16") \
-    X(MYNAH_K_FP8_256X256_BF16, "mynah_fp8_256x256_bf16") \
     X(MYNAH_K_TREE_F32, "mynah_tree_attn_f32_64_1x1") \
     X(MYNAH_K_TREE_F32_64_1X2, "mynah_tree_attn_f32_64_1x2") \
     X(MYNAH_K_TREE_F32_128_1X1, "mynah_tree_attn_f32_128_1x1") \

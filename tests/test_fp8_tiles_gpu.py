@@ -49,3 +49,53 @@ def test_few_blocks(M, monkeypatch, tile, rows, cols, tokens):
     want, s, _ = F.expected(w, ws, xq, xs)
     nb = ws.shape[1]
     assert np.all(np.abs(got - want) <= (128 + nb + 4) * U * s + E.rounded(want, E.F32))
+
+
+RAGGED = [(64, 128, 64), (129, 272, 65), (100, 1168, 130), (513, 912, 127), (1000, 640, 257),
+          (257, 2048, 300), (130, 144, 513)]
+
+
+@pytest.mark.parametrize("out", [E.F32, E.F16, E.BF16])
+@pytest.mark.parametrize("tile", range(4))
+@pytest.mark.parametrize("rows,cols,tokens", RAGGED)
+def test_tiles(M, monkeypatch, out, tile, rows, cols, tokens):
+    print("[case] fp8 tile", tile, out, rows, cols, tokens, flush=True)
+    monkeypatch.setenv("MYNAH_FP8_TILE", str(tile))
+    rng = np.random.default_rng(rows + 3 * cols + tokens)
+    w, ws, xq, xs = F.operands(rng, rows, cols, tokens)
+    got = product(M, w, ws, xq, xs, out)
+    want, s, _ = F.expected(w, ws, xq, xs)
+    sums = (128 + ws.shape[1] + 4) * U * s           # then one rounding to the type
+    assert np.all(np.abs(got - want) <= sums * (1 + E.HALF[out]) + E.rounded(want, out))
+
+
+def cancelling(rng, rows, cols, tokens):
+    """Whole numbers up to 8 beside two products of 448 x 448 and its negative in each
+    block: every sum in f32 is exact (below 2^24), scales are powers of two."""
+    nr, nb = -(-rows // 128), -(-cols // 128)
+    w = rng.integers(-8, 9, (rows, cols)).astype(np.float64)
+    x = rng.integers(-8, 9, (tokens, cols)).astype(np.float64)
+    for b in range(nb):
+        i, j = b * 128 + rng.choice(min(128, cols - b * 128), 2, replace=False)
+        x[:, i] = x[:, j] = 448
+        w[:, i] = 448
+        w[:, j] = -448
+    ws = np.full((nr, nb), 2.0 ** -3, np.float32)
+    xs = (2.0 ** rng.integers(-2, 3, (tokens, nb))).astype(np.float32)
+    return E.to_e4m3(w), ws, E.to_e4m3(x), xs
+
+
+@pytest.mark.parametrize("out", [E.F32, E.F16, E.BF16])
+@pytest.mark.parametrize("tile", [None, 0, 1, 2, 3])
+@pytest.mark.parametrize("tokens", [1, 16, 17, 64, 65, 300])
+def test_sums_that_cancel(M, monkeypatch, out, tile, tokens):
+    # Sums in 32 bits, whatever the type and the number of tokens.
+    rows, cols = 400, 400
+    print("[case] fp8 cancelling", tile, out, tokens, flush=True)
+    if tile is not None:
+        monkeypatch.setenv("MYNAH_FP8_TILE", str(tile))
+    w, ws, xq, xs = cancelling(np.random.default_rng(tokens), rows, cols, tokens)
+    want, s, _ = F.expected(w, ws, xq, xs)
+    assert np.abs(want).max() < 1e-2 * s.max()
+    got = product(M, w, ws, xq, xs, out)
+    assert np.all(np.abs(got - want) <= (0 if out == E.F32 else E.rounded(want, out)))
