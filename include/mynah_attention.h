@@ -68,7 +68,8 @@ int mynah_hip_rope_freqs(const mynah_rope_params *p, double *freqs, float *mscal
  * product and its reduction to one turn in 64 bits, so far positions keep
  * their angle; cos and sin in 32), scaled by mscale; the result is rounded
  * once to `type`. pos[t] may be negative (a rotation back); NULL: t itself.
- * y may be x with the same strides; otherwise they do not overlap.
+ * y may be x with the same strides; otherwise they do not overlap. Rows of y
+ * that overlap one another are refused; rows of x may (one for all tokens).
  * head_dim and rot_dim multiples of 8, rot_dim <= head_dim <= 512; tokens and
  * heads not 0. */
 int mynah_hip_rope_dev(int type, int layout, const void *x, size_t x_token, size_t x_head,
@@ -89,7 +90,8 @@ int mynah_hip_rope_dev(int type, int layout, const void *x, size_t x_token, size
  *     (padding rows of a batch); slots NULL: token t to slot t. The slots of a
  *     call are distinct: of two tokens with one slot, each value left there is
  *     one token's or the other's;
- *   - the outputs do not overlap the inputs. */
+ *   - the outputs do not overlap the inputs; strides that let rows of q_out or
+ *     slots overlap one another are refused. */
 typedef struct {
     int type, out_type, layout;
     uint32_t n_heads, n_kv_heads, head_dim, rot_dim;   /* as for mynah_hip_rope_dev */
@@ -135,6 +137,7 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  *     as they were, their keys unseen), positions past max_kv are unseen; rows
  *     of no sequence are left as they were, rows outside [0, n_rows) are not
  *     touched, and a negative n_past counts as 0;
+ *   - out overlaps none of the inputs;
  *   - head_dim 64, 128 or 256; 1 <= n_heads / n_kv_heads <= 64; page_size a
  *     power of two from 16 on; q, out, caches and strides aligned to 16 bytes;
  *     slot_stride below 2^24 bytes; max_kv <= 2^26, and with a mask max_nodes <= 32 *

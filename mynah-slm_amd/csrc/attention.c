@@ -123,6 +123,22 @@ static int fits(size_t n, size_t stride, size_t len, size_t size) {
     return stride <= (SIZE_MAX / 4 / size) / n && len <= SIZE_MAX / 4 / size;
 }
 
+/* Whether two of the rows at t * token + h * head, t < tokens, h < heads, of
+ * `len` elements each, share an element. Every size is one that
+ * fits() takes. */
+static int rows_meet(size_t tokens, size_t token, size_t heads, size_t head, size_t len) {
+    if ((tokens > 1 && token < len) || (heads > 1 && head < len)) return 1;
+    if (tokens == 1 || heads == 1 || token >= (heads - 1) * head + len ||
+        head >= (tokens - 1) * token + len)
+        return 0;
+    for (size_t h = 1; h < heads; h++)                  /* the tokens next to it */
+        for (size_t t = h * head / token, i = 0; i < 2 && t + i < tokens; i++) {
+            const size_t at = (t + i) * token, to = h * head;
+            if ((at > to ? at - to : to - at) < len) return 1;
+        }
+    return 0;
+}
+
 int mynah_hip_rope_dev(int type, int layout, const void *x, size_t x_token, size_t x_head,
                        void *y, size_t y_token, size_t y_head, size_t tokens, size_t heads,
                        uint32_t head_dim, uint32_t rot_dim, const double *freqs, float mscale,
@@ -137,6 +153,8 @@ int mynah_hip_rope_dev(int type, int layout, const void *x, size_t x_token, size
     if (!fits(tokens, x_token, head_dim, size) || !fits(heads, x_head, head_dim, size) ||
         !fits(tokens, y_token, head_dim, size) || !fits(heads, y_head, head_dim, size))
         return refuse("size overflow");
+    if (rows_meet(tokens, y_token, heads, y_head, head_dim))
+        return refuse("rope: rows of y overlap");
     if ((uintptr_t)x % size != 0 || (uintptr_t)y % size != 0 || (uintptr_t)freqs % 8 != 0 ||
         (uintptr_t)pos % 4 != 0)
         return refuse("rope: misaligned operand");
@@ -184,6 +202,9 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *p, void *stream) {
                 !fits(p->tokens, p->v_stride, nk * hd, size) ||
                 !fits(p->n_slots, p->slot_stride, nk * hd, out))))
         return refuse("size overflow");
+    if ((nq && rows_meet(p->tokens, p->q_out_stride, nq, hd, hd)) ||
+        (nk && rows_meet(p->n_slots, p->slot_stride, nk, hd, hd)))
+        return refuse("qk_norm_rope: rows of q_out or the caches overlap");
     if ((nq && ((uintptr_t)p->q % size != 0 || (uintptr_t)p->q_out % out != 0)) ||
         (nk && ((uintptr_t)p->k % size != 0 || (uintptr_t)p->v % size != 0 ||
                 (uintptr_t)p->k_cache % out != 0 || (uintptr_t)p->v_cache % out != 0)) ||
