@@ -84,3 +84,22 @@ def test_much_weight_in_small_probabilities(M, t, below):
     off = np.abs(got - want) / tol
     print(f"largest error {float(off.max()):.2f} of its bound", flush=True)
     assert off.max() <= 1
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_committed_keys_of_minus_infinity(M, t, hd):
+    """A committed key whose score is -inf is unseen in effect: the bound is that
+    of the call in which its page is no page."""
+    c = Tree(M, [(200, 6), (90, 2)], 4, 2, hd, t, page=16, seed=2)
+    for h in range(4):                                   # so that -inf times it is -inf
+        c.q[:, h * hd] = E.encode(np.abs(E.decode(c.q[:, h * hd], t)) + 0.5, t)
+    gone = [(0, 0), (0, 3), (0, 11), (1, 4)]
+    for b, p in gone:
+        rows = slice(int(c.pages[b, p]) * 16, int(c.pages[b, p]) * 16 + 16)
+        for h in range(2):
+            c.k[rows, h * hd] = E.encode(np.full(16, -np.inf), t)
+    raw = c.call()
+    for b, p in gone:
+        c.pages[b, p] = -1
+    c.check(raw)
