@@ -99,3 +99,36 @@ def test_sums_that_cancel(M, monkeypatch, out, tile, tokens):
     assert np.abs(want).max() < 1e-2 * s.max()
     got = product(M, w, ws, xq, xs, out)
     assert np.all(np.abs(got - want) <= (0 if out == E.F32 else E.rounded(want, out)))
+
+
+@pytest.mark.parametrize("long_side", ["rows", "tokens"])
+@pytest.mark.parametrize("tile", [None, 0, 2, 3])
+def test_offsets_past_32_bits(M, monkeypatch, long_side, tile):
+    """Weights, or activations, of over 4 GiB: the last rows, or tokens, are held to
+    their values; what lies before them is whatever the memory held."""
+    many, few, cols, tail = 1_050_000, 17 if tile is None else 70, 4112, 300
+    print("[case] fp8 offsets", long_side, tile, flush=True)
+    if tile is not None:
+        monkeypatch.setenv("MYNAH_FP8_TILE", str(tile))
+    nb, rng = -(-cols // 128), np.random.default_rng(4)
+    rows, tokens = (many, few) if long_side == "rows" else (few, many)
+    first = (many - tail) // 128 * 128                   # where a block of scales starts
+    tail = many - first
+    w, ws, xq, xs = F.operands(rng, tail if rows == many else rows, cols,
+                               tail if tokens == many else tokens)
+    nr = -(-rows // 128)
+    d = [M.DeviceBuffer(n) for n in (rows * cols, 4 * nr * nb, tokens * cols, 4 * tokens * nb)]
+    at = [first * cols, first // 128 * nb * 4, 0, 0] if rows == many else \
+        [0, 0, first * cols, first * nb * 4]
+    assert max(at) > 1 << 32
+    for b, o, a in zip(d, at, (w, ws, xq, xs)):
+        M.check(M.lib.mynah_hip_h2d(b.ptr + o, M.ptr(a), a.nbytes), "h2d")
+    y = M.DeviceBuffer(2 * rows * tokens)
+    M.fp8_matmat_dev(d[0].ptr, d[1].ptr, rows, cols, d[2].ptr, d[3].ptr, E.F16, y.ptr, tokens)
+    M.sync()
+    got = E.decode(y.download(np.float16, rows * tokens), E.F16).reshape(tokens, rows)
+    got = got[:, first:] if rows == many else got[first:]
+    want, s, _ = F.expected(w, ws, xq, xs)
+    ok = np.abs(want) + s < 60_000                       # f16 holds them
+    tol = (128 + nb + 4) * U * s * (1 + E.HALF[E.F16]) + E.rounded(want, E.F16)
+    assert ok.mean() > 0.9 and np.all(np.abs(got - want)[ok] <= tol[ok])
