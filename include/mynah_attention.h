@@ -127,7 +127,11 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  * the probabilities are rounded to the type for the product with V (f16: of n
  * positions, those below 2^-25 of the row's largest are off by n 2^-36 of it
  * together at most), the result once. The sums' order depends on the sizes,
- * max_* values and lengths alone, so equal calls give equal bits.
+ * max_* values and lengths alone, so equal calls give equal bits. Sequences are
+ * cut by their lengths over the CUs while n_seqs times n_kv_heads is below their
+ * number (times row groups, where a key head has more rows, max_nodes * group, than
+ * a workgroup takes: 32 in f32, 64 to 256 in 16 bits); from there on a sequence is
+ * not cut and the longest one sets the time.
  *   - position p of sequence b is cache row pages[b][p / page_size] * page_size
  *     + p % page_size, or without pages b * seq_slots + p; a row outside
  *     [0, n_slots) (a page id that is no page) is not read and counts as unseen;

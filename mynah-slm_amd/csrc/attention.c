@@ -324,10 +324,16 @@ static void tree_make_plan(const mynah_tree_attention *p, uint32_t cus, tree_pla
         t->rw = t->variant == 0u ? 1u : 1u << (t->variant - (t->nt == 2u));
     }
     t->groups = (uint32_t)((tiles + t->nt * t->rw - 1) / (t->nt * t->rw));
-    /* One workgroup fills a CU's LDS, so at most one for each CU: 264 on 256 CUs
-     * took 39 us where 240 take 22. Two or three workgroups a CU, one after the
-     * other, are slower too (16 sequences of up to 8207 bf16 positions cut alike 99,
-     * 109 and 121 us). */
+    /* At most one workgroup for each CU. A 128- or 256-wide one of one or two row
+     * waves fills its LDS: 264 on 256 CUs took 39 us where 240 take 22, and two or
+     * three a CU, one after the other, are slower too (16 sequences of up to 8207 bf16
+     * positions cut alike 99, 109 and 121 us). Two of head size 64 fit, and gain and
+     * lose: bf16, one node over 65,536 positions 43 us with two, 37 with one, the 16
+     * sequences 60 and 55; f32, 64 nodes over 130,000 586 and 657.
+     * So where sequences times key heads times row groups reach the CUs, nothing is
+     * cut, and the longest sequence has the call to itself: one of 32,768 bf16
+     * positions beside 15 of 512 47 us, beside 30 196 (one piece to spare), beside 31
+     * to 63 345 to 353. */
     const uint64_t base = (uint64_t)p->n_kv_heads * t->groups;
     const uint32_t turn = t->waves / t->rw * (f32 ? 16u : 32u) * (t->rw > 1 ? 2u : 1u);
     const uint64_t turns = (uint64_t)p->n_seqs * ((p->max_kv + turn - 1) / turn);

@@ -28,8 +28,8 @@ struct RopeArgs {
 // cos and sin of the angle p * f, scaled. The product and its reduction to an
 // eighth of a turn either side of a quarter are in double (a position of 2^31
 // keeps its angle to 2^-22 radians), the rest in f32: with |x| <= pi / 4 the
-// Taylor sums below end within 2e-9 (sin, next term x^11 / 11!) and 2e-9 (cos,
-// x^12 / 12!: 1.2e-10) of the functions, under their f32 rounding.
+// Taylor sums below end within 2e-9 (sin, next term x^11 / 11!) and 1.2e-10 (cos,
+// x^12 / 12!) of the functions, under their f32 rounding.
 MYNAH_DEV void turn(double p, double f, float mscale, float &c, float &s) {
     const double rev = p * f * 0.15915494309189535;       // 1 / (2 pi)
     const double r = rev - __builtin_rint(rev);

@@ -17,10 +17,10 @@
 // Bound by memory where a key head has few rows, by the matrix and exponential
 // units where it has many. Measured, MI355X: 16 sequences of up to 16 nodes and
 // 8207 bf16 positions in pages (32 heads, 8 of keys, 128 wide; 85,413 positions in all,
-// 350 MB) 96 us, 3.6 TB/s; the same with one node each 75 us, 4.7 TB/s; 64 nodes over 130,065 f16
-// positions (533 MB, 136 GFLOP) 206 us; one sequence of 16 nodes over 65,552 61 us,
-// 4.4 TB/s, of one node 53 us, 5.1 TB/s; 24 f32 nodes over 2072 positions 21 us; one
-// f32 token over 513 13 us.
+// 350 MB) 96 us, 3.6 TB/s; the same with one node each 80 us, 4.4 TB/s (75 without the
+// second launch); 64 nodes over 130,065 f16 positions (533 MB, 136 GFLOP) 203-213 us; one
+// sequence of 16 nodes over 65,552 69 us, 3.9 TB/s, of one node 62 us, 4.3 TB/s (56
+// without); 24 f32 nodes over 2072 positions 21 us; one f32 token over 513 13 us.
 //
 // SPDX-License-Identifier: MIT
 #pragma once
@@ -320,7 +320,8 @@ MYNAH_DEV void tree_attn(const TreeArgs &a) {
     const uint32_t end = sq.kv - begin < per ? sq.kv : begin + per;
 
     // What only the end or a mask needs waits in the LDS: in registers it would
-    // spill.
+    // spill (the 16-bit 128-wide kernels of two column tiles are at their limit, and
+    // keep two registers of their own in memory).
     if (threadIdx.x == 0u) {
         keep[0] = id;
         keep[1] = kvh;
