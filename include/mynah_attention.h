@@ -144,7 +144,8 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *a, void *stream);
  *   - out overlaps none of the inputs;
  *   - head_dim 64, 128 or 256; 1 <= n_heads / n_kv_heads <= 64; page_size a
  *     power of two from 16 on; q, out, caches and strides aligned to 16 bytes;
- *     slot_stride below 2^24 bytes; max_kv <= 2^26, and with a mask max_nodes <= 32 *
+ *     slot_stride below 2^24 bytes; n_seqs and n_heads <= 65536, max_nodes
+ *     <= 65535, max_kv <= 2^26, and with a mask max_nodes <= 32 *
  *     mask_words and n_rows * mask_words < 2^32. */
 typedef struct {
     int type;                                   /* of q, out and the caches */

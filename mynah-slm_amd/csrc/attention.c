@@ -79,8 +79,8 @@ static int seg_vec(const mynah_rope_seg *s, size_t in_size, size_t out_size) {
             (uintptr_t)s->in % (4u * in_size) == 0 && (uintptr_t)s->out % (4u * out_size) == 0);
 }
 
-static int rope_launch(mynah_device *d, int type, int out_type, int layout, mynah_rope_args *a,
-                       size_t tokens, hipStream_t st) {
+static int rope_launch(int type, int out_type, int layout, mynah_rope_args *a, size_t tokens,
+                       void *stream) {
     a->lanes_log2 = 0;
     while ((8u << a->lanes_log2) < a->hd) a->lanes_log2++;
     a->heads = a->seg[0].heads + a->seg[1].heads + a->seg[2].heads;
@@ -90,14 +90,16 @@ static int rope_launch(mynah_device *d, int type, int out_type, int layout, myna
     a->units = (unsigned long long)tokens * a->groups;
     const uint32_t per_wg = 256u >> a->lanes_log2;
     const unsigned long long wgs = (a->units + per_wg - 1) / per_wg;
-    if (wgs > 0x7fffffffu) return refuse("rope: too many rows for one launch");
+    if (wgs > MYNAH_MOST_WGS(256)) return refuse("rope: too many rows for one launch");
+    mynah_device *d = mynah_dev();
+    if (d == NULL) return -1;
     int vec = 1;
     for (int i = 0; i < 3; i++)
         vec &= seg_vec(&a->seg[i], elem_size(type), elem_size(out_type));
     uint32_t mode = (layout == MYNAH_ROPE_HALF ? 2u : 0u) | (uint32_t)vec;
     void *args[] = {a, &mode};
     return mynah_launch(d, MYNAH_K_ROPE + 3 * type_index(type) + type_index(out_type),
-                        (unsigned)wgs, 1, 256, 0, st, args);
+                        (unsigned)wgs, 1, 256, 0, mynah_stream_or_default(d, stream), args);
 }
 
 static int rope_shape(int layout, uint32_t head_dim, uint32_t rot_dim, size_t tokens,
@@ -158,8 +160,6 @@ int mynah_hip_rope_dev(int type, int layout, const void *x, size_t x_token, size
     if ((uintptr_t)x % size != 0 || (uintptr_t)y % size != 0 || (uintptr_t)freqs % 8 != 0 ||
         (uintptr_t)pos % 4 != 0)
         return refuse("rope: misaligned operand");
-    mynah_device *d = mynah_dev();
-    if (d == NULL) return -1;
     mynah_rope_args a;
     memset(&a, 0, sizeof a);
     a.seg[0].in = x;
@@ -175,7 +175,7 @@ int mynah_hip_rope_dev(int type, int layout, const void *x, size_t x_token, size
     a.hd = head_dim;
     a.rot = rot_dim;
     a.mscale = mscale;
-    return rope_launch(d, type, type, layout, &a, tokens, mynah_stream_or_default(d, stream));
+    return rope_launch(type, type, layout, &a, tokens, stream);
 }
 
 int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *p, void *stream) {
@@ -212,8 +212,6 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *p, void *stream) {
         (uintptr_t)p->freqs % 8 != 0 || (uintptr_t)p->pos % 4 != 0 ||
         (uintptr_t)p->slots % 4 != 0)
         return refuse("qk_norm_rope: misaligned operand");
-    mynah_device *d = mynah_dev();
-    if (d == NULL) return -1;
     mynah_rope_args a;
     memset(&a, 0, sizeof a);
     for (int i = 0; i < 3; i++) {
@@ -237,8 +235,7 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *p, void *stream) {
     a.rot = p->rot_dim;
     a.eps = p->eps;
     a.mscale = p->mscale;
-    return rope_launch(d, p->type, p->out_type, p->layout, &a, p->tokens,
-                       mynah_stream_or_default(d, stream));
+    return rope_launch(p->type, p->out_type, p->layout, &a, p->tokens, stream);
 }
 
 /* ── attention of drafted tokens over a cache ────────────────────────────── */
@@ -250,6 +247,8 @@ int mynah_hip_qk_norm_rope_dev(const mynah_qk_norm_rope *p, void *stream) {
 typedef struct {
     uint32_t variant, nt, rw, waves, groups, slots;
 } tree_plan;
+
+static void tree_make_plan(const mynah_tree_attention *p, uint32_t cus, tree_plan *t);
 
 static int tree_check(const mynah_tree_attention *p) {
     if (p == NULL || p->q == NULL || p->out == NULL || p->k_cache == NULL ||
@@ -296,6 +295,10 @@ static int tree_check(const mynah_tree_attention *p) {
           (uintptr_t)p->mask) & 3u) != 0)
         return refuse("tree_attention: q, out, caches and strides must be 16-byte aligned");
     if (!isfinite(p->scale)) return refuse("tree_attention: the scale must be finite");
+    tree_plan t;                                /* of whole sequences, the most there are */
+    tree_make_plan(p, 1, &t);
+    if ((uint64_t)p->n_seqs * p->n_kv_heads * t.groups > MYNAH_MOST_WGS(64 * t.waves))
+        return refuse("tree_attention: too many workgroups for one launch");
     return 0;
 }
 
@@ -425,7 +428,6 @@ int mynah_hip_tree_attention_dev(const mynah_tree_attention *p, void *workspace,
     if (p->scale < 0.0f) a.flip = p->type == MYNAH_F32 ? 0x80000000u : 0x80008000u;
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a};
-    if (wgs > 0x7fffffffu) return refuse("tree_attention: too many workgroups for one launch");
     if (mynah_launch(d, tree_kernel(p, t.variant), (unsigned)wgs, 1, 64 * t.waves, 0, st, args) != 0)
         return -1;
     if (t.slots == p->n_seqs) return 0;

@@ -47,7 +47,7 @@ int mynah_hip_fp8_quantize_dev(int type, const void *x, size_t x_stride, size_t 
     }
     uint32_t c32 = (uint32_t)cols, nb = (uint32_t)((cols + BLOCK - 1) / BLOCK);
     unsigned long long blocks = (unsigned long long)tokens * nb;
-    if ((blocks + 15) / 16 > 0x7fffffffu) {
+    if ((blocks + 15) / 16 > MYNAH_MOST_WGS(256)) {
         mynah_set_error("fp8: too many values for one launch");
         return -1;
     }
@@ -120,7 +120,7 @@ int mynah_hip_fp8_matmat_dev(const uint8_t *w, const float *ws, size_t rows, siz
         return -1;
     }
     if (check_shape(type, cols, tokens) != 0) return -1;
-    if (rows == 0 || rows > 0x7fffff00u || tokens > SIZE_MAX / 8 / rows) {
+    if (rows == 0 || (rows + 15) / 16 > MYNAH_MOST_WGS(256) || tokens > SIZE_MAX / 8 / rows) {
         mynah_set_error("fp8: bad row count");
         return -1;
     }
@@ -140,7 +140,7 @@ int mynah_hip_fp8_matmat_dev(const uint8_t *w, const float *ws, size_t rows, siz
     if (tl != NULL) {
         uint32_t tr = (uint32_t)((rows + tl->rows - 1) / tl->rows);
         const uint64_t wgs = (uint64_t)tr * ((tokens + tl->toks - 1) / tl->toks);
-        if (wgs <= 0x7fffffffu) {
+        if (wgs <= MYNAH_MOST_WGS(64 * tl->waves)) {
             void *args[] = {&w, &ws, &xq, &xs, &y, &r32, &c32, &t32, &nb, &tr};
             return mynah_launch(d, MYNAH_K_FP8_TILE + 3 * (int)(tl - fp8_tiles) + t, (unsigned)wgs, 1,
                                 64 * tl->waves, 0, st, args);

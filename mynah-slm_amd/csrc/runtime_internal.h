@@ -352,6 +352,10 @@ int mynah_gemv_prefetch_plan(const mynah_gemv_group *next, int order, uint32_t w
                              uint32_t bytes_per_wg, uint64_t max_bytes, uint32_t step_log2,
                              mynah_gemv_prefetch *pf);
 
+/* Workgroups of `threads` that one launch takes: its threads are counted in 32
+ * bits along a dimension. */
+#define MYNAH_MOST_WGS(threads) (UINT32_MAX / (threads))
+
 /* Host mirrors of rope.hip RopeSeg and RopeArgs. */
 typedef struct {
     const void *in;

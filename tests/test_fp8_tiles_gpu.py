@@ -132,3 +132,23 @@ def test_offsets_past_32_bits(M, monkeypatch, long_side, tile):
     ok = np.abs(want) + s < 60_000                       # f16 holds them
     tol = (128 + nb + 4) * U * s * (1 + E.HALF[E.F16]) + E.rounded(want, E.F16)
     assert ok.mean() > 0.9 and np.all(np.abs(got - want)[ok] <= tol[ok])
+
+
+@pytest.mark.parametrize("out", [E.F32, E.F16, E.BF16])
+@pytest.mark.parametrize("tokens", [3, 40, 200])
+def test_result_aligned_to_its_type_alone(M, out, tokens):
+    rows, cols = 256, 272
+    w, ws, xq, xs = F.operands(np.random.default_rng(6), rows, cols, tokens)
+    d = [M.DeviceBuffer.from_array(a) for a in (w, ws, xq, xs)]
+    y0 = E.encode(np.full(tokens * rows + 8, 5.0), out)
+    y, size = M.DeviceBuffer.from_array(y0), E.SIZE[out]
+    got = []
+    for at in (0, 1):
+        y.upload(y0)
+        M.fp8_matmat_dev(d[0].ptr, d[1].ptr, rows, cols, d[2].ptr, d[3].ptr, out,
+                         y.ptr + at * size, tokens)
+        M.sync()
+        raw = y.download(E.NP[out], y0.size)
+        got.append(raw[at:at + tokens * rows])
+        assert np.array_equal(np.delete(raw, np.s_[at:at + tokens * rows]), y0[:8])
+    assert np.array_equal(got[0].view(np.uint8), got[1].view(np.uint8))
