@@ -3,9 +3,8 @@
  * checks, launch geometry, the rotary frequency table.
  *
  * SPDX-License-Identifier: MIT */
-#include "mynah_attention.h"
+#include "args.h"
 #include "kernels_hip.h"
-#include "runtime_internal.h"
 
 #include <float.h>
 #include <math.h>
@@ -13,17 +12,6 @@
 #include <string.h>
 
 #define PI 3.14159265358979323846
-
-static int refuse(const char *what) {
-    mynah_set_error("%s", what);
-    return -1;
-}
-
-static size_t elem_size(int type) {
-    return type == MYNAH_F32 ? 4u : type == MYNAH_F16 || type == MYNAH_BF16 ? 2u : 0u;
-}
-
-static int type_index(int type) { return type == MYNAH_F32 ? 0 : type == MYNAH_F16 ? 1 : 2; }
 
 /* ── rotary positions ────────────────────────────────────────────────────── */
 
@@ -117,12 +105,6 @@ static int rope_shape(int layout, uint32_t head_dim, uint32_t rot_dim, size_t to
     if (tokens == 0 || heads == 0 || heads > 65536 || tokens > 0x7fffffffu)
         return refuse("rope: bad token or head count");
     return 0;
-}
-
-/* Whether `n` rows `stride` apart, of `len` elements each, fit the address
- * space in bytes. */
-static int fits(size_t n, size_t stride, size_t len, size_t size) {
-    return stride <= (SIZE_MAX / 4 / size) / n && len <= SIZE_MAX / 4 / size;
 }
 
 /* Whether two of the rows at t * token + h * head, t < tokens, h < heads, of

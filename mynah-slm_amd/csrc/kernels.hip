@@ -18,3 +18,4 @@
 #include "fp8.hip"
 #include "tree_attn.hip"
 #include "draft.hip"
+#include "kv8.hip"

@@ -192,7 +192,43 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_TREE_JOIN_F16_256, "mynah_tree_join_f16_256") \
     X(MYNAH_K_TREE_JOIN_BF16_64, "mynah_tree_join_bf16_64") \
     X(MYNAH_K_TREE_JOIN_BF16_128, "mynah_tree_join_bf16_128") \
-    X(MYNAH_K_TREE_JOIN_BF16_256, "mynah_tree_join_bf16_256")
+    X(MYNAH_K_TREE_JOIN_BF16_256, "mynah_tree_join_bf16_256") \
+    X(MYNAH_K_KV8_STORE, "mynah_kv8_store_f32_64_1") \
+    X(MYNAH_K_KV8_STORE_F32_64_4, "mynah_kv8_store_f32_64_4") \
+    X(MYNAH_K_KV8_STORE_F32_128_1, "mynah_kv8_store_f32_128_1") \
+    X(MYNAH_K_KV8_STORE_F32_128_4, "mynah_kv8_store_f32_128_4") \
+    X(MYNAH_K_KV8_STORE_F32_256_1, "mynah_kv8_store_f32_256_1") \
+    X(MYNAH_K_KV8_STORE_F32_256_4, "mynah_kv8_store_f32_256_4") \
+    X(MYNAH_K_KV8_STORE_F16_64_1, "mynah_kv8_store_f16_64_1") \
+    X(MYNAH_K_KV8_STORE_F16_64_4, "mynah_kv8_store_f16_64_4") \
+    X(MYNAH_K_KV8_STORE_F16_128_1, "mynah_kv8_store_f16_128_1") \
+    X(MYNAH_K_KV8_STORE_F16_128_4, "mynah_kv8_store_f16_128_4") \
+    X(MYNAH_K_KV8_STORE_F16_256_1, "mynah_kv8_store_f16_256_1") \
+    X(MYNAH_K_KV8_STORE_F16_256_4, "mynah_kv8_store_f16_256_4") \
+    X(MYNAH_K_KV8_STORE_BF16_64_1, "mynah_kv8_store_bf16_64_1") \
+    X(MYNAH_K_KV8_STORE_BF16_64_4, "mynah_kv8_store_bf16_64_4") \
+    X(MYNAH_K_KV8_STORE_BF16_128_1, "mynah_kv8_store_bf16_128_1") \
+    X(MYNAH_K_KV8_STORE_BF16_128_4, "mynah_kv8_store_bf16_128_4") \
+    X(MYNAH_K_KV8_STORE_BF16_256_1, "mynah_kv8_store_bf16_256_1") \
+    X(MYNAH_K_KV8_STORE_BF16_256_4, "mynah_kv8_store_bf16_256_4") \
+    X(MYNAH_K_KV8_ATTN, "mynah_kv8_attn_f32_i8_64") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_64, "mynah_kv8_attn_f32_e4m3_64") \
+    X(MYNAH_K_KV8_ATTN_F32_I8_128, "mynah_kv8_attn_f32_i8_128") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_128, "mynah_kv8_attn_f32_e4m3_128") \
+    X(MYNAH_K_KV8_ATTN_F32_I8_256, "mynah_kv8_attn_f32_i8_256") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_256, "mynah_kv8_attn_f32_e4m3_256") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_64, "mynah_kv8_attn_f16_i8_64") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_64, "mynah_kv8_attn_f16_e4m3_64") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_128, "mynah_kv8_attn_f16_i8_128") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_128, "mynah_kv8_attn_f16_e4m3_128") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_256, "mynah_kv8_attn_f16_i8_256") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_256, "mynah_kv8_attn_f16_e4m3_256") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_64, "mynah_kv8_attn_bf16_i8_64") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_64, "mynah_kv8_attn_bf16_e4m3_64") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_128, "mynah_kv8_attn_bf16_i8_128") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_128, "mynah_kv8_attn_bf16_e4m3_128") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_256, "mynah_kv8_attn_bf16_i8_256") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_256, "mynah_kv8_attn_bf16_e4m3_256")
 
 enum {
 #define X(id, name) id,
@@ -387,6 +423,25 @@ typedef struct {
     float scale2, lag;
     uint32_t flip;
 } mynah_tree_args;
+
+/* Host mirrors of kv8.hip Kv8StoreArgs and Kv8Args. */
+typedef struct {
+    const void *x[2];
+    size_t x_stride[2];
+    uint8_t *c[2];
+    float *s[2];
+    const int32_t *seq_start, *n_past, *pages;
+    size_t slot_stride, seq_slots;
+    unsigned long long n_slots, units;
+    uint32_t n_seqs, n_kv, n_rows, page_log2, max_pages, block_log2, blocks, max_nodes, max_kv;
+    uint32_t format;
+} mynah_kv8_store_args;
+typedef struct {
+    mynah_tree_args t;
+    const float *ks, *vs;
+    uint32_t block_log2;
+    float scale2;
+} mynah_kv8_args;
 
 /* Y[tokens][rows] = (res +) X[tokens][cols] · W^T in the matvec summation
  * order (every output bit-identical to the matvec of its token);

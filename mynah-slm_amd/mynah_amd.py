@@ -92,6 +92,33 @@ class TreeAttention(C.Structure):
                 ("scale", C.c_float)]
 
 
+class Kv8Cache(C.Structure):
+    """mynah_kv8_cache (include/mynah_cache.h); device addresses."""
+    _fields_ = [("format", C.c_int), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("block", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("slot_stride", C.c_size_t), ("n_slots", C.c_size_t), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("seq_slots", C.c_size_t), ("pages", C.c_void_p),
+                ("page_size", C.c_uint32), ("max_pages", C.c_uint32)]
+
+
+class Kv8Store(C.Structure):
+    """mynah_kv8_store (include/mynah_cache.h); device addresses."""
+    _fields_ = [("cache", Kv8Cache), ("type", C.c_int), ("n_seqs", C.c_uint32), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_stride", C.c_size_t), ("v_stride", C.c_size_t),
+                ("n_rows", C.c_uint32), ("seq_start", C.c_void_p), ("n_past", C.c_void_p),
+                ("max_nodes", C.c_uint32), ("max_kv", C.c_uint32)]
+
+
+class Kv8Attention(C.Structure):
+    """mynah_kv8_attention (include/mynah_cache.h); device addresses."""
+    _fields_ = [("cache", Kv8Cache), ("type", C.c_int), ("n_seqs", C.c_uint32),
+                ("n_heads", C.c_uint32), ("q", C.c_void_p), ("q_stride", C.c_size_t),
+                ("out", C.c_void_p), ("out_stride", C.c_size_t), ("n_rows", C.c_uint32),
+                ("seq_start", C.c_void_p), ("n_past", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_words", C.c_uint32), ("max_nodes", C.c_uint32), ("max_kv", C.c_uint32),
+                ("scale", C.c_float)]
+
+
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint32)
 
 
@@ -128,6 +155,9 @@ def _load() -> C.CDLL:
         "mynah_hip_qk_norm_rope_dev": (C.c_int, [C.POINTER(QkNormRope), _P]),
         "mynah_hip_tree_attention_workspace": (_SZ, [C.POINTER(TreeAttention)]),
         "mynah_hip_tree_attention_dev": (C.c_int, [C.POINTER(TreeAttention), _P, _SZ, _P]),
+        "mynah_hip_kv8_store_dev": (C.c_int, [C.POINTER(Kv8Store), _P]),
+        "mynah_hip_kv8_attention_workspace": (_SZ, [C.POINTER(Kv8Attention)]),
+        "mynah_hip_kv8_attention_dev": (C.c_int, [C.POINTER(Kv8Attention), _P, _SZ, _P]),
         "mynah_hip_init": (C.c_int, [C.c_int]),
         "mynah_hip_last_error": (C.c_char_p, []),
         "mynah_hip_register": (C.c_int, [_P, _SZ]),
@@ -461,6 +491,26 @@ def tree_attention_dev(args: TreeAttention, workspace: int, workspace_bytes: int
                        stream=None) -> None:
     check(lib.mynah_hip_tree_attention_dev(args, workspace, workspace_bytes, stream),
           "tree_attention")
+
+
+KV_I8, KV_E4M3 = 0, 1
+
+
+def kv8_store_dev(args: Kv8Store, stream=None) -> None:
+    check(lib.mynah_hip_kv8_store_dev(args, stream), "kv8_store")
+
+
+def kv8_attention_workspace(args: Kv8Attention) -> int:
+    n = int(lib.mynah_hip_kv8_attention_workspace(args))
+    if n == 0:
+        raise HipError(f"kv8_attention: {lib.mynah_hip_last_error().decode(errors='replace')}")
+    return n
+
+
+def kv8_attention_dev(args: Kv8Attention, workspace: int, workspace_bytes: int,
+                      stream=None) -> None:
+    check(lib.mynah_hip_kv8_attention_dev(args, workspace, workspace_bytes, stream),
+          "kv8_attention")
 
 
 def copy_dev(dst: int, src: int, nbytes: int, stream=None) -> None:
