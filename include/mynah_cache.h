@@ -139,6 +139,70 @@ size_t mynah_hip_kv8_attention_workspace(const mynah_kv8_attention *a);
 int mynah_hip_kv8_attention_dev(const mynah_kv8_attention *a, void *workspace,
                                 size_t workspace_bytes, void *stream);
 
+/* ── the pages of a cache ──────────────────────────────────────────────── */
+
+/* A part of a page: page p's is `bytes` bytes from base + p * stride on (a layer's
+ * keys, its values, their scales). Parts do not overlap. */
+typedef struct {
+    void *base;
+    size_t stride, bytes;
+} mynah_page_part;
+
+/* A pool of pages and the sequences that hold them. Sequence b's positions p lie in
+ * page pages[b][p / page_size], entries behind its pages are -1; several sequences
+ * may hold a page, refs[p] counts the table's entries that name page p, and a page
+ * of 0 is free. The calls keep that so. Everything is device memory and is read
+ * there, so a captured call follows it; the calls of a pool go one after the other
+ * (one stream, or events). Entries outside [0, n_pages) name no page.
+ * n_seqs <= 65536, n_parts <= 65534, n_seqs * max_pages and n_pages < 2^28,
+ * page_size a power of two. */
+typedef struct {
+    uint32_t n_pages, n_seqs, max_pages, page_size, n_parts;
+    const mynah_page_part *parts;               /* [n_parts] */
+    int32_t *refs;                              /* [n_pages] */
+    int32_t *pages;                             /* [n_seqs][max_pages] */
+    int32_t *n_past;                            /* [n_seqs]: positions held */
+    int32_t *status;                            /* [2] */
+} mynah_page_pool;
+
+/* Bytes of device workspace (aligned to 256 bytes) that a call of this pool needs;
+ * 0 with the reason in mynah_hip_last_error() where the pool is refused. */
+size_t mynah_hip_pages_workspace(const mynah_page_pool *p);
+
+/* Every sequence b becomes what sequence from[b] was before the call, or empty where
+ * from[b] is outside [0, n_seqs): its pages are shared, not copied, those that b held
+ * are given back. from[b] = b leaves b alone; any number may continue one (beams,
+ * samples of one prompt), in any order. */
+int mynah_hip_pages_fork_dev(const mynah_page_pool *p, const int32_t *from, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* Every sequence b gets pages of its own for positions n_past[b] .. n_past[b] +
+ * n_new[b] - 1 (n_new[b] <= 0: none are asked for): an entry there that names no page
+ * gets a free one, and one whose page others hold too gets a free one with, where it has
+ * positions before n_past[b], a copy of the page's content. If every holder of a page asks
+ * for it, the first keeps it. Free pages are given from the lowest on, in the order of
+ * sequences and positions. n_past stays as it is. status[0] is the number of pages
+ * that were missing, status[1] of sequences that would not fit max_pages entries: unless
+ * both are 0, nothing has changed. */
+int mynah_hip_pages_reserve_dev(const mynah_page_pool *p, const int32_t *n_new, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
+/* Every sequence b with keep[b] >= 0 is cut to at most keep[b] positions (0: it is
+ * gone), and pages that those do not need are given back, reserved ones too. */
+int mynah_hip_pages_release_dev(const mynah_page_pool *p, const int32_t *keep, void *stream);
+
+/* The n pages in use move into the pages 0 .. n - 1: each page from n on, in rising
+ * order, to the lowest free one, content, counts and table alike; what lies in the pages from n on
+ * is free. status[0] becomes n, status[1] the number of pages that moved. */
+int mynah_hip_pages_compact_dev(const mynah_page_pool *p, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
+/* The content of page from[i] to page to[i], i < n, all parts; the table and the
+ * counts stay. Pairs with an index outside [0, n_pages) are left out. No page is
+ * twice among `to`, nor in both. */
+int mynah_hip_pages_copy_dev(const mynah_page_pool *p, const int32_t *from, const int32_t *to,
+                             uint32_t n, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,3 +19,4 @@
 #include "tree_attn.hip"
 #include "draft.hip"
 #include "kv8.hip"
+#include "pages.hip"

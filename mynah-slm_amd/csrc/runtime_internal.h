@@ -228,7 +228,13 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_KV8_ATTN_BF16_I8_128, "mynah_kv8_attn_bf16_i8_128") \
     X(MYNAH_K_KV8_ATTN_BF16_E4M3_128, "mynah_kv8_attn_bf16_e4m3_128") \
     X(MYNAH_K_KV8_ATTN_BF16_I8_256, "mynah_kv8_attn_bf16_i8_256") \
-    X(MYNAH_K_KV8_ATTN_BF16_E4M3_256, "mynah_kv8_attn_bf16_e4m3_256")
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_256, "mynah_kv8_attn_bf16_e4m3_256") \
+    X(MYNAH_K_PAGES_FORK_TAKE, "mynah_pages_fork_take") \
+    X(MYNAH_K_PAGES_FORK_GIVE, "mynah_pages_fork_give") \
+    X(MYNAH_K_PAGES_RESERVE, "mynah_pages_reserve") \
+    X(MYNAH_K_PAGES_RELEASE, "mynah_pages_release") \
+    X(MYNAH_K_PAGES_COMPACT, "mynah_pages_compact") \
+    X(MYNAH_K_PAGES_MOVE, "mynah_pages_move")
 
 enum {
 #define X(id, name) id,
@@ -442,6 +448,15 @@ typedef struct {
     uint32_t block_log2;
     float scale2;
 } mynah_kv8_args;
+
+/* Host mirror of pages.hip PageArgs. */
+typedef struct {
+    uint32_t n_pages, n_seqs, max_pages, page_log2, n_parts, count;
+    const void *parts;
+    int32_t *refs, *pages, *n_past, *status;
+    const int32_t *ask, *from, *to;
+    int32_t *rows, *cnt, *first, *list, *moves, *map;
+} mynah_page_args;
 
 /* Y[tokens][rows] = (res +) X[tokens][cols] · W^T in the matvec summation
  * order (every output bit-identical to the matvec of its token);

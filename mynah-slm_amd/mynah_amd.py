@@ -119,6 +119,14 @@ class Kv8Attention(C.Structure):
                 ("scale", C.c_float)]
 
 
+class PagePool(C.Structure):
+    """mynah_page_pool (include/mynah_cache.h); device addresses."""
+    _fields_ = [("n_pages", C.c_uint32), ("n_seqs", C.c_uint32), ("max_pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_parts", C.c_uint32), ("parts", C.c_void_p),
+                ("refs", C.c_void_p), ("pages", C.c_void_p), ("n_past", C.c_void_p),
+                ("status", C.c_void_p)]
+
+
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint32)
 
 
@@ -158,6 +166,12 @@ def _load() -> C.CDLL:
         "mynah_hip_kv8_store_dev": (C.c_int, [C.POINTER(Kv8Store), _P]),
         "mynah_hip_kv8_attention_workspace": (_SZ, [C.POINTER(Kv8Attention)]),
         "mynah_hip_kv8_attention_dev": (C.c_int, [C.POINTER(Kv8Attention), _P, _SZ, _P]),
+        "mynah_hip_pages_workspace": (_SZ, [C.POINTER(PagePool)]),
+        "mynah_hip_pages_fork_dev": (C.c_int, [C.POINTER(PagePool), _P, _P, _SZ, _P]),
+        "mynah_hip_pages_reserve_dev": (C.c_int, [C.POINTER(PagePool), _P, _P, _SZ, _P]),
+        "mynah_hip_pages_release_dev": (C.c_int, [C.POINTER(PagePool), _P, _P]),
+        "mynah_hip_pages_compact_dev": (C.c_int, [C.POINTER(PagePool), _P, _SZ, _P]),
+        "mynah_hip_pages_copy_dev": (C.c_int, [C.POINTER(PagePool), _P, _P, C.c_uint32, _P]),
         "mynah_hip_init": (C.c_int, [C.c_int]),
         "mynah_hip_last_error": (C.c_char_p, []),
         "mynah_hip_register": (C.c_int, [_P, _SZ]),
@@ -511,6 +525,38 @@ def kv8_attention_dev(args: Kv8Attention, workspace: int, workspace_bytes: int,
                       stream=None) -> None:
     check(lib.mynah_hip_kv8_attention_dev(args, workspace, workspace_bytes, stream),
           "kv8_attention")
+
+
+def pages_workspace(pool: PagePool) -> int:
+    n = int(lib.mynah_hip_pages_workspace(pool))
+    if n == 0:
+        raise HipError(f"pages: {lib.mynah_hip_last_error().decode(errors='replace')}")
+    return n
+
+
+def pages_fork_dev(pool: PagePool, source: int, workspace: int, workspace_bytes: int,
+                   stream=None) -> None:
+    check(lib.mynah_hip_pages_fork_dev(pool, source, workspace, workspace_bytes, stream),
+          "pages_fork")
+
+
+def pages_reserve_dev(pool: PagePool, n_new: int, workspace: int, workspace_bytes: int,
+                      stream=None) -> None:
+    check(lib.mynah_hip_pages_reserve_dev(pool, n_new, workspace, workspace_bytes, stream),
+          "pages_reserve")
+
+
+def pages_release_dev(pool: PagePool, keep: int, stream=None) -> None:
+    check(lib.mynah_hip_pages_release_dev(pool, keep, stream), "pages_release")
+
+
+def pages_compact_dev(pool: PagePool, workspace: int, workspace_bytes: int, stream=None) -> None:
+    check(lib.mynah_hip_pages_compact_dev(pool, workspace, workspace_bytes, stream),
+          "pages_compact")
+
+
+def pages_copy_dev(pool: PagePool, source: int, to: int, n: int, stream=None) -> None:
+    check(lib.mynah_hip_pages_copy_dev(pool, source, to, n, stream), "pages_copy")
 
 
 def copy_dev(dst: int, src: int, nbytes: int, stream=None) -> None:

@@ -84,3 +84,44 @@ def test_launches_too_large():
     assert "too many workgroups" in refused_attn(
         {"pages": None, "seq_slots": 128, "n_kv_heads": 512, "slot_stride": 65536}, n_seqs=65536,
         n_heads=512, q_stride=65536, out_stride=65536)
+
+
+# ── pages ────────────────────────────────────────────────────────────────────
+
+POOL = dict(n_pages=8, n_seqs=3, max_pages=4, page_size=16, n_parts=2, parts=P, refs=P, pages=P,
+            n_past=P, status=P)
+BIG = 1 << 30
+
+
+@pytest.mark.parametrize("change", [
+    {"n_pages": 0}, {"n_pages": 1 << 28}, {"n_seqs": 0}, {"n_seqs": 65537}, {"max_pages": 0},
+    {"max_pages": 1 << 27}, {"page_size": 0}, {"page_size": 24}, {"n_parts": 0}, {"n_parts": 65535},
+    {"parts": None}, {"refs": None}, {"pages": None}, {"n_past": None}, {"status": None},
+    {"parts": P + 4}, {"refs": P + 2}, {"status": P + 1}], ids=str)
+def test_pool_refused(change):
+    a = C.byref(M.PagePool(**{**POOL, **change}))
+    lib = M.lib
+    assert lib.mynah_hip_pages_workspace(a) == 0 and error()
+    assert lib.mynah_hip_pages_fork_dev(a, P, P, BIG, None) == -1
+    assert lib.mynah_hip_pages_reserve_dev(a, P, P, BIG, None) == -1
+    assert lib.mynah_hip_pages_release_dev(a, P, None) == -1
+    assert lib.mynah_hip_pages_compact_dev(a, P, BIG, None) == -1
+    assert lib.mynah_hip_pages_copy_dev(a, P, P, 1, None) == -1
+
+
+def test_pool_arguments_refused():
+    a, lib = C.byref(M.PagePool(**POOL)), M.lib
+    need = lib.mynah_hip_pages_workspace(a)
+    assert need >= 4 * (3 * 5 + 6 * 8 + 1)
+    for x in (None, P + 2):
+        assert lib.mynah_hip_pages_fork_dev(a, x, P, BIG, None) == -1
+        assert lib.mynah_hip_pages_reserve_dev(a, x, P, BIG, None) == -1
+        assert lib.mynah_hip_pages_release_dev(a, x, None) == -1
+        assert lib.mynah_hip_pages_copy_dev(a, x, P, 1, None) == -1
+        assert lib.mynah_hip_pages_copy_dev(a, P, x, 1, None) == -1
+    assert lib.mynah_hip_pages_copy_dev(a, P, P, 0, None) == -1
+    for ws, n in ((None, need), (P + 16, need), (P, need - 1)):
+        assert lib.mynah_hip_pages_fork_dev(a, P, ws, n, None) == -1 and "workspace" in error()
+        assert lib.mynah_hip_pages_reserve_dev(a, P, ws, n, None) == -1
+        assert lib.mynah_hip_pages_compact_dev(a, ws, n, None) == -1
+    assert lib.mynah_hip_pages_workspace(None) == 0
