@@ -117,6 +117,50 @@ int mynah_hip_sampler_accept(mynah_hip_sampler *s, uint32_t token);
  * generation loop samples on the device without this host copy. 0, or -1. */
 int mynah_hip_sample(mynah_hip_sampler *s, float *logits, uint32_t *id);
 
+/* ── rules on a batch's logits, ahead of any choice ───────────────────────────
+ * No reference counterpart for a batch (its sampler penalises one sequence's logits,
+ * src/sampler.c:72-94). For every row r and token i, in 32 bits, in this order:
+ *   penalties  where i occurs c > 0 times in the row's history hist[hist_start[r]] ..
+ *              hist[hist_start[r + 1] - 1]:
+ *                l = l > 0 ? l / repeat[r] : l * repeat[r]
+ *                l = l - freq[r] * c
+ *                l = l - presence[r]
+ *              MYNAH_PENALTY_ONCE: once for the token; MYNAH_PENALTY_EACH: c times over, as
+ *              the sampler above does for its window (the same bits); NULL arrays
+ *              stand for 1, 0 and 0
+ *   biases     l = l + bias[k] where bias_id[k] = i, bias_start[r] <= k < bias_start[r +
+ *              1]; of several such k the last
+ *   grammars   -inf unless bit i % 32 of allowed[m][i / 32] is set, m = mask_row[r] (NULL: r);
+ *              a row with m outside [0, n_masks) has none
+ * rounded to out_type once. Ids outside [0, vocab) count for nothing. All pointers are device
+ * pointers and everything but the sizes is read there, so a captured call follows it; calls are
+ * asynchronous on `stream`, allocate nothing. hist, bias_id and allowed may be NULL: no
+ * such rule. Starts rise and are 64-bit counts. Types are ggml's ids F32 = 0, F16 = 1, BF16 = 30;
+ * strides count elements; y may be x with the same type and stride, otherwise they do not
+ * overlap. mask_words >= ceil(vocab / 32); vocab < 2^31; elements on their own
+ * size. 0, or -1 with the reason in mynah_hip_last_error(). */
+enum { MYNAH_PENALTY_ONCE = 0, MYNAH_PENALTY_EACH = 1 };
+typedef struct {
+    int type, out_type;
+    uint32_t n_rows, vocab;
+    const void *x;
+    size_t x_stride;
+    void *y;
+    size_t y_stride;
+    const int32_t *hist;
+    const int64_t *hist_start;                  /* [n_rows + 1] */
+    const float *repeat, *freq, *presence;      /* [n_rows] */
+    int penalty;
+    const int32_t *bias_id;
+    const float *bias;
+    const int64_t *bias_start;                  /* [n_rows + 1] */
+    const uint32_t *allowed;                    /* [n_masks][mask_words] */
+    const int32_t *mask_row;                    /* [n_rows] */
+    uint32_t mask_words, n_masks;
+} mynah_logits;
+
+int mynah_hip_logits_dev(const mynah_logits *a, void *stream);
+
 /* src/generate.h:47-52 (mynah_slm_generate). t may be NULL. */
 long mynah_hip_qwen3_generate_tokens(mynah_qwen3 *s, const mynah_hip_gen_params *p,
                                      mynah_hip_timing *t);

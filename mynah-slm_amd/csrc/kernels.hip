@@ -20,3 +20,4 @@
 #include "draft.hip"
 #include "kv8.hip"
 #include "pages.hip"
+#include "logits.hip"

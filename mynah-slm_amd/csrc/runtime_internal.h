@@ -234,7 +234,16 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_PAGES_RESERVE, "mynah_pages_reserve") \
     X(MYNAH_K_PAGES_RELEASE, "mynah_pages_release") \
     X(MYNAH_K_PAGES_COMPACT, "mynah_pages_compact") \
-    X(MYNAH_K_PAGES_MOVE, "mynah_pages_move")
+    X(MYNAH_K_PAGES_MOVE, "mynah_pages_move") \
+    X(MYNAH_K_LOGITS, "mynah_logits_f32_f32") \
+    X(MYNAH_K_LOGITS_F32_F16, "mynah_logits_f32_f16") \
+    X(MYNAH_K_LOGITS_F32_BF16, "mynah_logits_f32_bf16") \
+    X(MYNAH_K_LOGITS_F16_F32, "mynah_logits_f16_f32") \
+    X(MYNAH_K_LOGITS_F16_F16, "mynah_logits_f16_f16") \
+    X(MYNAH_K_LOGITS_F16_BF16, "mynah_logits_f16_bf16") \
+    X(MYNAH_K_LOGITS_BF16_F32, "mynah_logits_bf16_f32") \
+    X(MYNAH_K_LOGITS_BF16_F16, "mynah_logits_bf16_f16") \
+    X(MYNAH_K_LOGITS_BF16_BF16, "mynah_logits_bf16_bf16")
 
 enum {
 #define X(id, name) id,
@@ -244,6 +253,9 @@ enum {
 };
 
 #define MYNAH_MAX_DEVICES 16
+
+/* Tokens per workgroup of the rules on logits (= LG_CH in logits.hip). */
+#define MYNAH_LOGITS_CH 8192u
 
 /* Quads of values per thread of the dequantiser (= DQ_STEP in dequant.hip). */
 #define MYNAH_DQ_STEP 4u
@@ -457,6 +469,22 @@ typedef struct {
     const int32_t *ask, *from, *to;
     int32_t *rows, *cnt, *first, *list, *moves, *map;
 } mynah_page_args;
+
+/* Host mirror of logits.hip LogitsArgs. */
+typedef struct {
+    const void *x;
+    void *y;
+    size_t x_stride, y_stride;
+    const int32_t *hist;
+    const int64_t *hist_start;
+    const float *repeat, *freq, *presence;
+    const int32_t *bias_id;
+    const float *bias;
+    const int64_t *bias_start;
+    const uint32_t *allowed;
+    const int32_t *mask_row;
+    uint32_t vocab, chunks, mask_words, n_masks, each, vec;
+} mynah_logits_args;
 
 /* Y[tokens][rows] = (res +) X[tokens][cols] · W^T in the matvec summation
  * order (every output bit-identical to the matvec of its token);

@@ -127,6 +127,17 @@ class PagePool(C.Structure):
                 ("status", C.c_void_p)]
 
 
+class Logits(C.Structure):
+    """mynah_logits (include/mynah_generate.h); device addresses."""
+    _fields_ = [("type", C.c_int), ("out_type", C.c_int), ("n_rows", C.c_uint32),
+                ("vocab", C.c_uint32), ("x", C.c_void_p), ("x_stride", C.c_size_t),
+                ("y", C.c_void_p), ("y_stride", C.c_size_t), ("hist", C.c_void_p),
+                ("hist_start", C.c_void_p), ("repeat", C.c_void_p), ("freq", C.c_void_p),
+                ("presence", C.c_void_p), ("penalty", C.c_int), ("bias_id", C.c_void_p),
+                ("bias", C.c_void_p), ("bias_start", C.c_void_p), ("allowed", C.c_void_p),
+                ("mask_row", C.c_void_p), ("mask_words", C.c_uint32), ("n_masks", C.c_uint32)]
+
+
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint32)
 
 
@@ -172,6 +183,7 @@ def _load() -> C.CDLL:
         "mynah_hip_pages_release_dev": (C.c_int, [C.POINTER(PagePool), _P, _P]),
         "mynah_hip_pages_compact_dev": (C.c_int, [C.POINTER(PagePool), _P, _SZ, _P]),
         "mynah_hip_pages_copy_dev": (C.c_int, [C.POINTER(PagePool), _P, _P, C.c_uint32, _P]),
+        "mynah_hip_logits_dev": (C.c_int, [C.POINTER(Logits), _P]),
         "mynah_hip_init": (C.c_int, [C.c_int]),
         "mynah_hip_last_error": (C.c_char_p, []),
         "mynah_hip_register": (C.c_int, [_P, _SZ]),
@@ -557,6 +569,13 @@ def pages_compact_dev(pool: PagePool, workspace: int, workspace_bytes: int, stre
 
 def pages_copy_dev(pool: PagePool, source: int, to: int, n: int, stream=None) -> None:
     check(lib.mynah_hip_pages_copy_dev(pool, source, to, n, stream), "pages_copy")
+
+
+PENALTY_ONCE, PENALTY_EACH = 0, 1
+
+
+def logits_dev(args: Logits, stream=None) -> None:
+    check(lib.mynah_hip_logits_dev(args, stream), "logits")
 
 
 def copy_dev(dst: int, src: int, nbytes: int, stream=None) -> None:
