@@ -125,20 +125,23 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *p, void *stream) {
 
 /* ── attention ───────────────────────────────────────────────────────────── */
 
-/* What a call launches: a workgroup of `waves` waves for each key head, group of
- * `rows` query rows and slot: a sequence's, or with more slots than sequences a
- * piece of one. */
+/* What a call launches: kernel family `wide` or not, a workgroup of 8 waves for each
+ * key head, group of `rows` query rows and slot: a sequence's, or with more slots
+ * than sequences a piece of one. */
 typedef struct {
-    uint32_t rows, waves, groups, slots;
+    uint32_t wide, rows, groups, slots;
 } kv8_plan;
+#define KV8_WAVES 8u
 
 static void make_plan(const mynah_kv8_attention *p, uint32_t cus, kv8_plan *t) {
     const uint32_t group = p->n_heads / p->cache.n_kv_heads;
-    t->rows = 16;
-    t->waves = 8;
-    t->groups = (uint32_t)(((uint64_t)p->max_nodes * group + t->rows - 1) / t->rows);
+    const uint64_t rows = (uint64_t)p->max_nodes * group;
+    t->wide = rows > 64u;
+    t->rows = !t->wide ? 16u : p->type == MYNAH_F32 || p->cache.head_dim == 256 ? 128u : 256u;
+    t->groups = (uint32_t)((rows + t->rows - 1) / t->rows);
     const uint64_t base = (uint64_t)p->cache.n_kv_heads * t->groups;
-    const uint32_t turn = t->waves * (p->cache.head_dim == 256 ? 32u : 64u);
+    const uint32_t chunk = p->cache.head_dim == 256 ? 32u : 64u;
+    const uint32_t turn = t->wide ? chunk : KV8_WAVES * chunk;
     const uint64_t turns = (uint64_t)p->n_seqs * ((p->max_kv + turn - 1) / turn);
     uint64_t s = cus / base;
     if (s > turns) s = turns;
@@ -180,7 +183,7 @@ static int attn_check(const mynah_kv8_attention *p) {
     if (!isfinite(p->scale)) return refuse("kv8_attention: the scale must be finite");
     kv8_plan t;                                 /* of whole sequences, the most there are */
     make_plan(p, 1, &t);
-    if ((uint64_t)p->n_seqs * c->n_kv_heads * t.groups > MYNAH_MOST_WGS(64 * t.waves))
+    if ((uint64_t)p->n_seqs * c->n_kv_heads * t.groups > MYNAH_MOST_WGS(64 * KV8_WAVES))
         return refuse("kv8_attention: too many workgroups for one launch");
     return 0;
 }
@@ -260,8 +263,8 @@ int mynah_hip_kv8_attention_dev(const mynah_kv8_attention *p, void *workspace,
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a}, *join[] = {&a.t};
     const int h = c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2, ti = type_index(p->type);
-    if (mynah_launch(d, MYNAH_K_KV8_ATTN + 6 * ti + 2 * h + c->format, (unsigned)wgs, 1,
-                     64 * t.waves, 0, st, args) != 0)
+    if (mynah_launch(d, (t.wide ? MYNAH_K_KV8_WIDE : MYNAH_K_KV8_ATTN) + 6 * ti + 2 * h + c->format, (unsigned)wgs, 1,
+                     64 * KV8_WAVES, 0, st, args) != 0)
         return -1;
     if (t.slots == p->n_seqs) return 0;
     return mynah_launch3(d, MYNAH_K_TREE_JOIN + 3 * ti + h, p->n_seqs, p->max_nodes,

@@ -280,6 +280,114 @@ MYNAH_DEV uint32_t kv8_round(float x, float y) {        // to bf16
     return as_u32(v2b{(__bf16)x, (__bf16)y});
 }
 
+// The eight dimensions at q of a query as operands: step k of each of its numbers.
+template <class T, int QN, int K>
+MYNAH_DEV void kv8_query(const T *q, bool live, uint32_t flip, uint32_t (&qv)[QN][K][4], int k) {
+    constexpr int D = sizeof(T) == 4 ? 8 : 4;
+    uint32_t d[D];
+    *(uint4 *)d = *(const uint4 *)q;
+    if constexpr (D == 8) *(uint4 *)(d + 4) = *(const uint4 *)(q + 4);
+#pragma unroll
+    for (int i = 0; i < D; i++) d[i] = live ? d[i] ^ flip : 0u;
+    if constexpr (D == 8) {
+        float v[8];
+        __builtin_memcpy(v, d, 32);
+#pragma unroll
+        for (int t = 0; t < 3; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) qv[t][k][i] = kv8_cut(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) qv[0][k][i] = d[i];
+    }
+}
+
+// A column's scores of TILES tiles, four a lane, to weights: running maximum m, sum l
+// and outputs o follow. References are in log2 units; fma takes a score's difference to
+// its column's in one rounding. They lag by up to 2^8 in the probabilities.
+template <class T, int TILES, int VE, int PN>
+MYNAH_DEV void kv8_weigh(const float (&s)[TILES][4], const float (&ks)[TILES],
+                         const float (&vs)[TILES], float &m, float &l, ta_v4f (&o)[VE],
+                         uint32_t (&w)[TILES / 2][PN][4]) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+        top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])) * ks[t]);
+    if (__any(top - m > 8.0f)) {
+        top = fmaxf(m, lane_max4(top));
+        const float f = exp2_hw(m - (top == -INFINITY ? 0.0f : top));
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < VE; e++) o[e] *= f;
+        m = top;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int t = 0; t < TILES; t++) {
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            p[r] = exp2_hw(fmaf(s[t][r], ks[t], -base));
+            l += p[r];
+            p[r] *= vs[t];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int n = 0; n < PN; n++)
+                w[t / 2][n][2 * (t % 2) + i] =
+                    n == PN - 1 ? kv8_round(p[2 * i], p[2 * i + 1]) : kv8_cut(p[2 * i], p[2 * i + 1]);
+    }
+}
+
+// Which of the CK <= 64 positions from c on (uniform) a query sees, as bits: node
+// `node` of its sequence, its words of the mask from `words` on. Positions past the
+// sequence's last are for the caller to leave out.
+MYNAH_DEV uint64_t kv8_sees(const TreeArgs &a, size_t words, uint32_t node, uint32_t past,
+                            uint32_t c) {
+    const long long off = (long long)c - past;     // the first one's node
+    if (!a.mask) {
+        const long long n = (long long)node + 1 - off;
+        return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1u;
+    }
+    auto word = [&](uint32_t i) -> uint64_t { return i < a.mask_words ? a.mask[words + i] : 0u; };
+    if (off < 0) {
+        const uint32_t n = off < -64 ? 64u : (uint32_t)-off;
+        return n >= 64u ? ~0ull : (word(0) | word(1) << 32) << n | ((1ull << n) - 1u);
+    }
+    const uint32_t i = (uint32_t)off / 32u, sh = (uint32_t)off % 32u;
+    const uint64_t low = word(i) | word(i + 1u) << 32;
+    return sh ? low >> sh | word(i + 2u) << (64u - sh) : low;
+}
+// Bits of the positions that tiles of n[t] rows have.
+template <int TILES>
+MYNAH_DEV uint64_t kv8_there(const uint32_t (&n)[TILES]) {
+    uint64_t b = 0u;
+#pragma unroll
+    for (int t = 0; t < TILES; t++) b |= (uint64_t)((1u << n[t]) - 1u) << (16 * t);
+    return b;
+}
+// Scores of positions without their bit (the lane's first at bit 0) become -inf.
+template <int TILES>
+MYNAH_DEV void kv8_hide(float (&s)[TILES][4], uint64_t bits) {
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[t][r] = bits >> (16 * t + r) & 1u ? s[t][r] : -INFINITY;
+}
+
+// Four rows of four bytes, turned.
+MYNAH_DEV void kv8_turn(const uint32_t (&x)[4], uint32_t (&y)[4]) {
+    const uint32_t p0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);
+    const uint32_t p1 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+    const uint32_t p2 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+    const uint32_t p3 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+    y[0] = __builtin_amdgcn_perm(p2, p0, 0x05040100u);
+    y[1] = __builtin_amdgcn_perm(p2, p0, 0x07060302u);
+    y[2] = __builtin_amdgcn_perm(p3, p1, 0x05040100u);
+    y[3] = __builtin_amdgcn_perm(p3, p1, 0x07060302u);
+}
+
 // A workgroup's W waves take chunks of CK keys in turn, for the same 16 queries,
 // straight from memory into registers: a chunk's keys are under way while the one
 // before is weighed, its values while its scores are made. The waves' results meet
@@ -325,30 +433,11 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
     const bool live = rr < rows && qrow >= 0 && qrow < (long long)a.n_rows;
     const size_t words = live ? (size_t)qrow * a.mask_words : 0;
     uint32_t qv[S::QN][2 * S::KP][4];
-    {
-        const T *q = (const T *)a.q + (live ? (size_t)qrow * a.q_stride : 0) +
-                     (size_t)(kvh * a.group + rr - node * a.group) * HD;
+    const T *q = (const T *)a.q + (live ? (size_t)qrow * a.q_stride : 0) +
+                 (size_t)(kvh * a.group + rr - node * a.group) * HD;
 #pragma unroll
-        for (int k = 0; k < 2 * S::KP; k++) {
-            const T *p = q + 16u * (lk + 4u * (k / 2)) + 8u * (k % 2);
-            uint32_t d[S::F32 ? 8 : 4];
-            *(uint4 *)d = *(const uint4 *)p;
-            if constexpr (S::F32) *(uint4 *)(d + 4) = *(const uint4 *)(p + 4);
-#pragma unroll
-            for (int i = 0; i < (S::F32 ? 8 : 4); i++) d[i] = live ? d[i] ^ a.flip : 0u;
-            if constexpr (S::F32) {
-                float v[8];
-                __builtin_memcpy(v, d, 32);
-#pragma unroll
-                for (int t = 0; t < 3; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) qv[t][k][i] = kv8_cut(v[2 * i], v[2 * i + 1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) qv[0][k][i] = d[i];
-            }
-        }
-    }
+    for (int k = 0; k < 2 * S::KP; k++)
+        kv8_query<T>(q + 16u * (lk + 4u * (k / 2)) + 8u * (k % 2), live, a.flip, qv, k);
     float m = -INFINITY, l = 0.0f;
     ta_v4f o[S::VE];
 #pragma unroll
@@ -458,54 +547,19 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
         if (!whole) {
             // The nodes' chunk, the last, one with a bad page: unseen positions score
             // -inf, and a node's values that are NaN become zeros.
+            kv8_hide(s, (kv8_sees(a, words, node, sq.past, c) & kv8_there(cnv)) >> (4u * lk));
+            if constexpr (F == KV_E4M3)
 #pragma unroll
-            for (int t = 0; t < S::TILES; t++)
+                for (int t = 0; t < S::TILES; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint32_t i = 4u * lk + r, p = c + 16u * t + i;
-                    const uint32_t j = p < sq.past ? 0u : p - sq.past;
-                    const uint32_t ok = sees_node(a, words, node, j < sq.nodes ? j : sq.nodes - 1u) |
-                                        (uint32_t)(p < sq.past);
-                    s[t][r] = (ok & (uint32_t)(i < cnv[t])) ? s[t][r] : -INFINITY;
-                    if constexpr (F == KV_E4M3)
+                    for (int r = 0; r < 4; r++)
 #pragma unroll
                         for (int d = 0; d < S::VD; d++)
-                            vr[t][r][d] = p < sq.past ? vr[t][r][d] : kv8_no_nan(vr[t][r][d]);
-                }
+                            vr[t][r][d] = c + 16u * t + 4u * lk + r < sq.past
+                                              ? vr[t][r][d] : kv8_no_nan(vr[t][r][d]);
         }
-        // References are in log2 units; fma takes a score's difference to its column's
-        // in one rounding. They lag by up to 2^8 in the probabilities.
-        float top = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < S::TILES; t++)
-            top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])) * cks[t]);
-        if (__any(top - m > 8.0f)) {
-            top = fmaxf(m, lane_max4(top));
-            const float f = exp2_hw(m - (top == -INFINITY ? 0.0f : top));
-            l *= f;
-#pragma unroll
-            for (int e = 0; e < S::VE; e++) o[e] *= f;
-            m = top;
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
         uint32_t w[S::TILES / 2][S::PN][4];
-#pragma unroll
-        for (int t = 0; t < S::TILES; t++) {
-            float p[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                p[r] = exp2_hw(fmaf(s[t][r], cks[t], -base));
-                l += p[r];
-                p[r] *= cvs[t];
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int n = 0; n < S::PN; n++)
-                    w[t / 2][n][2 * (t % 2) + i] = n == S::PN - 1
-                                                       ? kv8_round(p[2 * i], p[2 * i + 1])
-                                                       : kv8_cut(p[2 * i], p[2 * i + 1]);
-        }
+        kv8_weigh<T, S::TILES, S::VE>(s, cks, cvs, m, l, o, w);
         // Values: four keys' bytes of one dimension side by side, then widened.
 #pragma unroll
         for (int u = 0; u < S::TILES / 2; u++)
@@ -514,15 +568,9 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                 uint32_t y[2][4];
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const uint32_t(&x)[4][S::VD] = vr[2 * u + t];
-                    const uint32_t p0 = __builtin_amdgcn_perm(x[1][d], x[0][d], 0x05010400u);
-                    const uint32_t p1 = __builtin_amdgcn_perm(x[1][d], x[0][d], 0x07030602u);
-                    const uint32_t p2 = __builtin_amdgcn_perm(x[3][d], x[2][d], 0x05010400u);
-                    const uint32_t p3 = __builtin_amdgcn_perm(x[3][d], x[2][d], 0x07030602u);
-                    y[t][0] = __builtin_amdgcn_perm(p2, p0, 0x05040100u);
-                    y[t][1] = __builtin_amdgcn_perm(p2, p0, 0x07060302u);
-                    y[t][2] = __builtin_amdgcn_perm(p3, p1, 0x05040100u);
-                    y[t][3] = __builtin_amdgcn_perm(p3, p1, 0x07060302u);
+                    const uint32_t x[4] = {vr[2 * u + t][0][d], vr[2 * u + t][1][d],
+                                           vr[2 * u + t][2][d], vr[2 * u + t][3][d]};
+                    kv8_turn(x, y[t]);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -597,9 +645,304 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
     }
 }
 
+// ── many rows ───────────────────────────────────────────────────────────────
+//
+// A prompt's rows: the workgroup's waves share a chunk of CK keys, each with 16 NT
+// rows of its own. Every code is widened once a workgroup: a chunk's codes come into registers
+// while the one before is computed, and leave for the LDS as bf16 (keys of f16 calls
+// f16), the values turned so that a lane reads eight keys of one dimension. Two
+// buffers, one barrier a chunk. Places in the LDS are 16-byte pieces, swapped so that
+// the eight lanes of an access meet no bank twice.
+template <class T, int HD>
+struct Kv8Wide {
+    using S = Kv8Shape<T, HD>;
+    static constexpr int W = 8;
+    static constexpr int NT = S::F32 || HD == 256 ? 1 : 2;  // column tiles of a wave
+    static constexpr int ROWS = 16 * NT * W;
+    static constexpr int CK = HD == 256 ? 32 : 64, TILES = CK / 16;
+    static constexpr int KS = HD / 32;              // steps of a score's product
+    static constexpr int LB = HD == 64 ? 8 : 16;    // bytes of a thread's keys
+    static constexpr int PR = CK / 8;               // pieces of a dimension's keys
+};
+
+template <class T, int F, int HD>
+MYNAH_DEV void kv8_wide(const Kv8Args &g) {
+    using S = Kv8Shape<T, HD>;
+    using Z = Kv8Wide<T, HD>;
+    constexpr int NT = Z::NT, TILES = Z::TILES;
+    const TreeArgs &a = g.t;
+    __shared__ uint4 kl[2][Z::CK * HD / 8], vl[2][Z::CK * HD / 8];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63u, lm = lane & 15u, lk = lane >> 4;
+    uint32_t id = blockIdx.x;
+    const uint32_t even = gridDim.x & ~7u;
+    if (id < even) id = (id & 7u) * (even >> 3) + (id >> 3);
+    const uint32_t head_id = id / a.groups, slot = head_id / a.n_kv;
+    const uint32_t kvh = head_id - slot * a.n_kv, grp = id - head_id * a.groups;
+    SlotShare share = {slot, 0u, ~0u};
+    if (a.slots > a.n_seqs) {                      // uniform
+        if (a.n_seqs == 1u) share = {0u, slot, 0u};
+        else if (!share_slots(a, slot, Z::CK, kvh == 0u && grp == 0u, share)) return;
+    }
+    const uint32_t b = __builtin_amdgcn_readfirstlane(share.b);
+    const uint32_t split = __builtin_amdgcn_readfirstlane(share.split);
+    const SeqSpan sq = seq_span(a, b);
+    const uint32_t rows = sq.nodes * a.group, wg0 = grp * Z::ROWS;
+    if (wg0 >= rows) return;                       // uniform
+    uint32_t per = __builtin_amdgcn_readfirstlane(share.per);
+    if (per == 0u) {
+        per = (sq.kv + a.slots - 1u) / a.slots;
+        per = (per + Z::CK - 1u) / Z::CK * Z::CK;
+    }
+    const unsigned long long from = (unsigned long long)split * per;
+    const uint32_t begin = from < sq.kv ? (uint32_t)from : sq.kv;
+    uint32_t end = sq.kv - begin < per ? sq.kv : begin + per;
+    // The last position that a chain's rows see, of the workgroup and of the wave.
+    const bool chain = a.mask == nullptr;
+    const uint32_t w0 = wg0 + 16u * NT * wave;
+    auto sees_upto = [&](uint32_t r) {
+        const unsigned long long p = (unsigned long long)sq.past + (r < rows ? r : rows - 1u) / a.group + 1u;
+        return p < end ? (uint32_t)p : end;
+    };
+    uint32_t mine = end;
+    if (chain) {
+        mine = w0 < rows ? sees_upto(w0 + 16u * NT - 1u) : begin;
+        const uint32_t all = sees_upto(wg0 + Z::ROWS - 1u);
+        end = all > begin ? all : begin;
+    }
+    const uint32_t first_node = (w0 < rows ? w0 : rows - 1u) / a.group;
+
+    // Each wave's own: its columns' nodes, and their first words of the mask. In
+    // registers they would spill.
+    __shared__ uint32_t lnode[Z::W][16 * NT], lwords[Z::W][16 * NT];
+    uint32_t qv[NT][S::QN][Z::KS][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const uint32_t rr = w0 + 16u * n + lm;
+        const uint32_t nd = rr / a.group;
+        const long long qrow = sq.row0 + nd;
+        const bool live = rr < rows && qrow >= 0 && qrow < (long long)a.n_rows;
+        lnode[wave][16 * n + lm] = nd;
+        lwords[wave][16 * n + lm] = live ? (uint32_t)qrow * a.mask_words : 0u;
+        const T *q = (const T *)a.q + (live ? (size_t)qrow * a.q_stride : 0) +
+                     (size_t)(kvh * a.group + rr - nd * a.group) * HD;
+#pragma unroll
+        for (int k = 0; k < Z::KS; k++) kv8_query<T>(q + 32u * k + 8u * lk, live, a.flip, qv[n], k);
+    }
+    float m[NT], l[NT];
+    ta_v4f o[NT][S::VE];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < S::VE; e++) o[n][e] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // A thread's part of a chunk: LB bytes of key tk, and four keys from 4 tv on of
+    // four dimensions from td on.
+    const uint32_t tk = threadIdx.x / (HD / Z::LB), tp = threadIdx.x % (HD / Z::LB);
+    const uint32_t tv = threadIdx.x / (HD / 4), td = threadIdx.x % (HD / 4) * 4u;
+    const bool has_v = tv < Z::CK / 4;
+    const uint32_t sb = (uint32_t)a.slot_stride;
+    const uint8_t *kbase = (const uint8_t *)a.k + (size_t)kvh * HD;
+    const uint8_t *vbase = (const uint8_t *)a.v + (size_t)kvh * HD;
+    uint32_t kc[4], vc[4];
+    // The 16 rows of the tile at position p.
+    auto tile = [&](const uint8_t *base, uint32_t p) {
+        unsigned long long r = 0;
+        uint32_t n = 0;
+        if (p < end && cache_row(a, b, p, r)) n = end - p < 16u ? end - p : 16u;
+        else r = 0;
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(base + r * sb), 0, n * sb, 0x00020000);
+    };
+    auto load = [&](uint32_t c) {
+        const uint32_t k16 = __builtin_amdgcn_readfirstlane(tk & ~15u);
+        const uint32_t v16 = __builtin_amdgcn_readfirstlane(4u * tv & ~15u);
+        const auto kb = tile(kbase, c + k16);
+        const uint32_t at = __umul24(tk & 15u, sb) + Z::LB * tp;
+        if constexpr (Z::LB == 16) {
+            const kv8_v4u x = __builtin_amdgcn_raw_buffer_load_b128(kb, at, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) kc[i] = x[i];
+        } else {
+            const kv8_v2u x = __builtin_amdgcn_raw_buffer_load_b64(kb, at, 0, 0);
+            kc[0] = x[0];
+            kc[1] = x[1];
+        }
+        if (has_v) {
+            const auto vb = tile(vbase, c + v16);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                vc[r] = __builtin_amdgcn_raw_buffer_load_b32(vb, __umul24((4u * tv & 15u) + r, sb) + td,
+                                                             0, 0);
+        }
+    };
+    // Widened into the LDS. Key k's piece p (eight dimensions) lies at place p ^ (k &
+    // 7) of its row; keys 16 t + 4 i .. + 3 of dimension d are half t & 1 of piece
+    // 4 (t / 2) + i of d's row, at place piece ^ turn(d).
+    auto turn = [](uint32_t d) { return Z::PR == 8 ? d & 7u : (d >> 2) & 3u; };
+    auto widen = [&](uint32_t c, int buf) {
+#pragma unroll
+        for (int p = 0; p < Z::LB / 8; p++) {
+            uint4 w;
+            if constexpr (S::F16) {
+                kv8_f16<F>(kc[2 * p], w.x, w.y);
+                kv8_f16<F>(kc[2 * p + 1], w.z, w.w);
+            } else {
+                kv8_bf16<F>(kc[2 * p], w.x, w.y);
+                kv8_bf16<F>(kc[2 * p + 1], w.z, w.w);
+            }
+            kl[buf][tk * (HD / 8) + ((Z::LB / 8 * tp + p) ^ (tk & 7u))] = w;
+        }
+        if (has_v) {
+            if constexpr (F == KV_E4M3)
+#pragma unroll
+                for (int r = 0; r < 4; r++)        // a node's NaN is 0
+                    vc[r] = c + 4u * tv + r < sq.past ? vc[r] : kv8_no_nan(vc[r]);
+            uint32_t y[4];
+            kv8_turn(vc, y);
+            const uint32_t t = tv / 4u, piece = t / 2u * 4u + (tv & 3u);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint2 w;
+                kv8_bf16<F>(y[i], w.x, w.y);
+                const uint32_t d = td + i;
+                *((uint2 *)&vl[buf][d * Z::PR + (piece ^ turn(d))] + (t & 1u)) = w;
+            }
+        }
+    };
+
+    float ks[TILES], vs[TILES];
+    uint32_t cnv[TILES];
+    auto scales = [&](uint32_t c) {
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            const uint32_t p = c + 16u * t;
+            unsigned long long r;
+            cnv[t] = 0;
+            ks[t] = vs[t] = 0.0f;
+            if (p >= end || !cache_row(a, b, p, r)) continue;
+            cnv[t] = end - p < 16u ? end - p : 16u;
+            const size_t at = (size_t)(r >> g.block_log2) * a.n_kv + kvh;
+            const float k = scalar_f32(g.ks, at), v = scalar_f32(g.vs, at);
+            ks[t] = k < INFINITY ? k : 0.0f;
+            vs[t] = v > 0.0f && v < INFINITY ? v : 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; t++)
+            ks[t] = fminf(fmaxf(ks[t] * g.scale2, 1e-30f), 3.402823466e38f);
+    };
+    // The lane's places: of piece 4 k + lk of key lm, and of 4 u + lk of dimension lm.
+    const uint32_t kat[2] = {lm * (HD / 8) + (lk ^ (lm & 7u)), lm * (HD / 8) + ((4u + lk) ^ (lm & 7u))};
+    uint32_t vat[TILES / 2];
+#pragma unroll
+    for (int u = 0; u < TILES / 2; u++) vat[u] = lm * Z::PR + ((4u * u + lk) ^ turn(lm));
+    auto compute = [&](uint32_t c, int buf) {
+        float s[NT][TILES][4];
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            ta_v4f x[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) x[n] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < Z::KS; k++) {
+                const uint4 kk = kl[buf][kat[k % 2] + 16 * t * (HD / 8) + 8 * (k / 2)];
+                const uint32_t w[4] = {kk.x, kk.y, kk.z, kk.w};
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = S::QN - 1; i >= 0; i--) {
+                        if constexpr (S::F16) x[n] = ta_mfma<_Float16>(w, qv[n][i][k], x[n]);
+                        else x[n] = ta_mfma<__bf16>(w, qv[n][i][k], x[n]);
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[n][t][r] = x[n][r];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        bool whole = c + Z::CK <= sq.past + (chain ? first_node : 0u);
+#pragma unroll
+        for (int t = 0; t < TILES; t++) whole = whole && cnv[t] == 16u;
+        if (!whole) {
+            const uint64_t there = kv8_there(cnv);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                kv8_hide(s[n], (kv8_sees(a, lwords[wave][16 * n + lm], lnode[wave][16 * n + lm],
+                                         sq.past, c) & there) >> (4u * lk));
+        }
+        uint32_t w[NT][TILES / 2][S::PN][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            kv8_weigh<T, TILES, S::VE>(s[n], ks, vs, m[n], l[n], o[n], w[n]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int u = 0; u < TILES / 2; u++)
+#pragma unroll
+            for (int e = 0; e < S::VE; e++) {
+                const uint4 vv = vl[buf][vat[u] + 16 * e * Z::PR];
+                const uint32_t va[4] = {vv.x, vv.y, vv.z, vv.w};
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = S::PN - 1; i >= 0; i--)
+                        o[n][e] = ta_mfma<__bf16>(va, w[n][u][i], o[n][e]);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    load(begin);
+    widen(begin, 0);
+    __syncthreads();
+    for (uint32_t c = begin; c < end; c += 2u * Z::CK) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t at = c + h * Z::CK;
+            load(at + Z::CK);
+            if (at < mine) {
+                scales(at);
+                compute(at, h);
+            }
+            widen(at + Z::CK, 1 - h);
+            __syncthreads();
+        }
+    }
+
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const float all = lane_sum4(l[n]);
+        const uint32_t rr = w0 + 16u * n + lm;
+        const uint32_t nd = rr / a.group;
+        const long long orow = sq.row0 + nd;
+        if (rr >= rows || orow < 0 || orow >= (long long)a.n_rows) continue;
+        const size_t at = (size_t)id * Z::ROWS + (rr - wg0);
+        const bool joined = a.slots > a.n_seqs;
+        if (joined && lk == 0u) {
+            a.pm[at] = m[n];
+            a.pl[at] = all;
+        }
+        const float inv = 1.0f / all;
+        T *y = (T *)a.out + (size_t)orow * a.out_stride +
+               (size_t)(kvh * a.group + rr - nd * a.group) * HD;
+#pragma unroll
+        for (int e = 0; e < S::VE; e++) {
+            const uint32_t d = 16u * e + 4u * lk;
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = joined ? o[n][e][r] : all == 0.0f ? 0.0f : o[n][e][r] * inv;
+            if (joined) *(float4 *)(a.po + at * HD + d) = float4{v[0], v[1], v[2], v[3]};
+            else store4<true>(y + d, v);
+        }
+    }
+}
+
 #define KV8_ATTN(name, T, fmt, F, HD)                                                        \
     extern "C" __global__ void __launch_bounds__((64 * Kv8Shape<T, HD>::W), 2)               \
-        mynah_kv8_attn_##name##_##fmt##_##HD(Kv8Args a) { kv8_attn<T, F, HD>(a); }
+        mynah_kv8_attn_##name##_##fmt##_##HD(Kv8Args a) { kv8_attn<T, F, HD>(a); }           \
+    extern "C" __global__ void __launch_bounds__((64 * Kv8Wide<T, HD>::W), 2)                \
+        mynah_kv8_wide_##name##_##fmt##_##HD(Kv8Args a) { kv8_wide<T, F, HD>(a); }
 #define KV8_ATTNS(name, T, HD) \
     KV8_ATTN(name, T, i8, KV_I8, HD) KV8_ATTN(name, T, e4m3, KV_E4M3, HD)
 KV8_ATTNS(f32, float, 64)
