@@ -248,10 +248,10 @@ MYNAH_DEV void kv8_f16(uint32_t c, uint32_t &lo, uint32_t &hi) {
     }
 }
 
-// Bytes that are e4m3's NaN as zeros.
-MYNAH_DEV uint32_t kv8_no_nan(uint32_t d) {
-    const uint32_t n = ((d & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // bit 7 of such a byte
-    return d & ~((n >> 7) * 0xffu);
+// Bytes that are e4m3's NaN as zeros (of either sign), of those with bit 7 of `which`.
+MYNAH_DEV uint32_t kv8_no_nan(uint32_t d, uint32_t which) {
+    const uint32_t n = ((d & 0x7f7f7f7fu) + 0x01010101u) & which;
+    return d & ~(n - (n >> 7));
 }
 
 template <class T, int HD>
@@ -302,42 +302,53 @@ MYNAH_DEV void kv8_query(const T *q, bool live, uint32_t flip, uint32_t (&qv)[QN
     }
 }
 
-// A column's scores of TILES tiles, four a lane, to weights: running maximum m, sum l
-// and outputs o follow. References are in log2 units; fma takes a score's difference to
-// its column's in one rounding. They lag by up to 2^8 in the probabilities.
-template <class T, int TILES, int VE, int PN>
-MYNAH_DEV void kv8_weigh(const float (&s)[TILES][4], const float (&ks)[TILES],
-                         const float (&vs)[TILES], float &m, float &l, ta_v4f (&o)[VE],
-                         uint32_t (&w)[TILES / 2][PN][4]) {
-    float top = -INFINITY;
+// A column's scores of TILES tiles, four a lane, become weights in two steps. First
+// its reference, m, follows the largest; sum l and outputs o with it. References are
+// in log2 units and lag by up to 2^8 in the probabilities.
+template <int NT, int TILES, int VE>
+MYNAH_DEV void kv8_refer(const float (&s)[NT][TILES][4], const float (&ks)[TILES], float (&m)[NT],
+                         float (&l)[NT], ta_v4f (&o)[NT][VE]) {
+    float top[NT];
+    bool grown = false;
 #pragma unroll
-    for (int t = 0; t < TILES; t++)
-        top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])) * ks[t]);
-    if (__any(top - m > 8.0f)) {
-        top = fmaxf(m, lane_max4(top));
-        const float f = exp2_hw(m - (top == -INFINITY ? 0.0f : top));
-        l *= f;
+    for (int n = 0; n < NT; n++) {
+        top[n] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < VE; e++) o[e] *= f;
-        m = top;
+        for (int t = 0; t < TILES; t++)
+            top[n] = fmaxf(top[n], fmaxf(fmaxf(s[n][t][0], s[n][t][1]),
+                                         fmaxf(s[n][t][2], s[n][t][3])) * ks[t]);
+        grown = grown || top[n] - m[n] > 8.0f;
     }
+    if (!__any(grown)) return;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const float to = fmaxf(m[n], lane_max4(top[n]));
+        const float f = exp2_hw(m[n] - (to == -INFINITY ? 0.0f : to));
+        l[n] *= f;
+#pragma unroll
+        for (int e = 0; e < VE; e++) o[n][e] *= f;
+        m[n] = to;
+    }
+}
+// Then a tile's four scores become weights, rounded as two dwords of each of their PN
+// numbers: fma takes a score's difference to the reference in one rounding.
+template <int PN>
+MYNAH_DEV void kv8_weigh(const float (&s)[4], float ks, float vs, float m, float &l,
+                         uint32_t (&w)[PN][4], int half) {
     const float base = m == -INFINITY ? 0.0f : m;
+    float p[4];
 #pragma unroll
-    for (int t = 0; t < TILES; t++) {
-        float p[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            p[r] = exp2_hw(fmaf(s[t][r], ks[t], -base));
-            l += p[r];
-            p[r] *= vs[t];
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int n = 0; n < PN; n++)
-                w[t / 2][n][2 * (t % 2) + i] =
-                    n == PN - 1 ? kv8_round(p[2 * i], p[2 * i + 1]) : kv8_cut(p[2 * i], p[2 * i + 1]);
+    for (int r = 0; r < 4; r++) {
+        p[r] = exp2_hw(fmaf(s[r], ks, -base));
+        l += p[r];
+        p[r] *= vs;
     }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int n = 0; n < PN; n++)
+            w[n][2 * half + i] =
+                n == PN - 1 ? kv8_round(p[2 * i], p[2 * i + 1]) : kv8_cut(p[2 * i], p[2 * i + 1]);
 }
 
 // Which of the CK <= 64 positions from c on (uniform) a query sees, as bits: node
@@ -359,12 +370,13 @@ MYNAH_DEV uint64_t kv8_sees(const TreeArgs &a, size_t words, uint32_t node, uint
     const uint64_t low = word(i) | word(i + 1u) << 32;
     return sh ? low >> sh | word(i + 2u) << (64u - sh) : low;
 }
-// Bits of the positions that tiles of n[t] rows have.
+// Bits of the positions that tiles have, lane t's of n rows.
 template <int TILES>
-MYNAH_DEV uint64_t kv8_there(const uint32_t (&n)[TILES]) {
+MYNAH_DEV uint64_t kv8_there(uint32_t n) {
     uint64_t b = 0u;
 #pragma unroll
-    for (int t = 0; t < TILES; t++) b |= (uint64_t)((1u << n[t]) - 1u) << (16 * t);
+    for (int t = 0; t < TILES; t++)
+        b |= (uint64_t)((1u << __builtin_amdgcn_readlane(n, t)) - 1u) << (16 * t);
     return b;
 }
 // Scores of positions without their bit (the lane's first at bit 0) become -inf.
@@ -387,6 +399,68 @@ MYNAH_DEV void kv8_turn(const uint32_t (&x)[4], uint32_t (&y)[4]) {
     y[2] = __builtin_amdgcn_perm(p3, p1, 0x05040100u);
     y[3] = __builtin_amdgcn_perm(p3, p1, 0x07060302u);
 }
+
+// Where a chunk's tiles of 16 positions lie: each lane has tile lane % TILES, and hands
+// it out by readlane. What a chunk needs is read ahead in two steps, its pages' ids,
+// then, from those, its scales, so that no wave waits for one read after the other.
+// (As scalars the tiles took 200 scalar instructions a chunk and spilled.)
+MYNAH_DEV uint32_t lane_of(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+MYNAH_DEV float lane_of(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+struct Kv8Tile {
+    unsigned long long row;         // the first cache row
+    uint32_t n;                     // how many of the 16 there are
+};
+template <int TILES>
+struct Kv8Walk {
+    const Kv8Args &g;
+    uint32_t b, kvh, end, at;       // sequence, key head, positions' end, the lane's 16 t
+    __device__ __forceinline__ Kv8Walk(const Kv8Args &g_, uint32_t b_, uint32_t kvh_, uint32_t end_)
+        : g(g_), b(b_), kvh(kvh_), end(end_), at(threadIdx.x % TILES * 16u) {}
+    __device__ __forceinline__ int32_t page(uint32_t c) const {
+        if (!g.t.pages) return 0;
+        const uint32_t p = c + at < end ? c + at : end - 1u;
+        return g.t.pages[(size_t)b * g.t.max_pages + (p >> g.t.page_log2)];
+    }
+    __device__ __forceinline__ Kv8Tile tile(uint32_t c, int32_t id) const {
+        const uint32_t p = c + at, low = p & ((1u << g.t.page_log2) - 1u);
+        Kv8Tile x;
+        x.row = g.t.pages ? ((unsigned long long)(uint32_t)id << g.t.page_log2) + low
+                          : (unsigned long long)b * g.t.seq_slots + p;
+        const bool there = p < end && id >= 0 && x.row < g.t.n_slots;   // whole blocks
+        x.row = there ? x.row : 0u;
+        x.n = !there ? 0u : end - p < 16u ? end - p : 16u;
+        return x;
+    }
+    __device__ __forceinline__ void scales(const Kv8Tile &x, float &k, float &v) const {
+        const size_t i = (size_t)(x.row >> g.block_log2) * g.t.n_kv + kvh;
+        k = g.ks[i];
+        v = g.vs[i];
+    }
+    // As the products take them: the keys' times the call's, in log2 units; 0 unless
+    // positive and finite (the keys' next to it, so that -inf stays what it is).
+    __device__ __forceinline__ void settle(float k, float v, float (&ks)[TILES],
+                                           float (&vs)[TILES]) const {
+        k = fminf(fmaxf((k < INFINITY ? k : 0.0f) * g.scale2, 1e-30f), 3.402823466e38f);
+        v = v > 0.0f && v < INFINITY ? v : 0.0f;
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            ks[t] = lane_of(k, t);
+            vs[t] = lane_of(v, t);
+        }
+    }
+    // The buffer of tile t (uniform) of rows of sb bytes: rows past its last are out of
+    // range, are not read and become zeros.
+    __device__ __forceinline__ auto buffer(const uint8_t *base, uint32_t sb, const Kv8Tile &x,
+                                           int t) const {
+        const unsigned long long row =
+            (unsigned long long)lane_of((uint32_t)(x.row >> 32), t) << 32 | lane_of((uint32_t)x.row, t);
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(base + row * sb), 0, lane_of(x.n, t) * sb,
+                                                 0x00020000);
+    }
+};
 
 // A workgroup's W waves take chunks of CK keys in turn, for the same 16 queries,
 // straight from memory into registers: a chunk's keys are under way while the one
@@ -438,87 +512,70 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
 #pragma unroll
     for (int k = 0; k < 2 * S::KP; k++)
         kv8_query<T>(q + 16u * (lk + 4u * (k / 2)) + 8u * (k % 2), live, a.flip, qv, k);
-    float m = -INFINITY, l = 0.0f;
-    ta_v4f o[S::VE];
+    float m[1] = {-INFINITY}, l[1] = {0.0f};
+    ta_v4f o[1][S::VE];
 #pragma unroll
-    for (int e = 0; e < S::VE; e++) o[e] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int e = 0; e < S::VE; e++) o[0][e] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // Tiles of the next chunk: the first cache row, how many of the 16 there are,
-    // their scales (the keys' times the call's, in log2 units).
     const uint32_t sb = (uint32_t)a.slot_stride;
     const uint8_t *kbase = (const uint8_t *)a.k + (size_t)kvh * HD;
     const uint8_t *vbase = (const uint8_t *)a.v + (size_t)kvh * HD;
-    unsigned long long row[S::TILES];
-    uint32_t nv[S::TILES], cnv[S::TILES];
-    float ks[S::TILES], vs[S::TILES], cks[S::TILES], cvs[S::TILES];
-    auto find = [&](uint32_t c) {
-#pragma unroll
-        for (int t = 0; t < S::TILES; t++) {
-            const uint32_t p = c + 16u * t;
-            row[t] = 0;
-            nv[t] = 0;
-            ks[t] = vs[t] = 0.0f;
-            unsigned long long r;
-            if (p >= end || !cache_row(a, b, p, r)) continue;
-            row[t] = r;
-            nv[t] = end - p < 16u ? end - p : 16u;   // n_slots is whole blocks
-            const size_t at = (size_t)(r >> g.block_log2) * a.n_kv + kvh;
-            ks[t] = scalar_f32(g.ks, at);
-            vs[t] = scalar_f32(g.vs, at);
-        }
-    };
+    const Kv8Walk<S::TILES> walk(g, b, kvh, end);
+    Kv8Tile x;                                     // of the chunk to be loaded
+    int32_t ahead;                                 // the page of the one after it
+    float ks[S::TILES], vs[S::TILES], nks, nvs;
     kv8_v4u kr[S::TILES][S::KP];
     uint32_t vr[S::TILES][4][S::VD];
     // Rows past a tile's last are out of its buffer's range, are not read and
     // become zeros.
-    auto rsrc = [&](const uint8_t *base, int t) {
-        return __builtin_amdgcn_make_buffer_rsrc((void *)(base + row[t] * sb), 0, nv[t] * sb,
-                                                 0x00020000);
-    };
     auto load_k = [&]() {
 #pragma unroll
-        for (int t = 0; t < S::TILES; t++)
+        for (int t = 0; t < S::TILES; t++) {
+            const auto kb = walk.buffer(kbase, sb, x, t);
 #pragma unroll
             for (int h = 0; h < S::KP; h++)
                 kr[t][h] = __builtin_amdgcn_raw_buffer_load_b128(
-                    rsrc(kbase, t), __umul24(lm, sb) + 16u * lk, 64 * h, 0);
+                    kb, __umul24(lm, sb) + 16u * lk, 64 * h, 0);
+        }
     };
     auto load_v = [&]() {
 #pragma unroll
-        for (int t = 0; t < S::TILES; t++)
+        for (int t = 0; t < S::TILES; t++) {
+            const auto vb = walk.buffer(vbase, sb, x, t);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const uint32_t at = __umul24(4u * lk + r, sb) + S::VE * lm;
                 if constexpr (S::VD == 1) {
-                    vr[t][r][0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc(vbase, t), at, 0, 0);
+                    vr[t][r][0] = __builtin_amdgcn_raw_buffer_load_b32(vb, at, 0, 0);
                 } else if constexpr (S::VD == 2) {
-                    const kv8_v2u x = __builtin_amdgcn_raw_buffer_load_b64(rsrc(vbase, t), at, 0, 0);
+                    const kv8_v2u x = __builtin_amdgcn_raw_buffer_load_b64(vb, at, 0, 0);
                     vr[t][r][0] = x[0];
                     vr[t][r][1] = x[1];
                 } else {
-                    const kv8_v4u x = __builtin_amdgcn_raw_buffer_load_b128(rsrc(vbase, t), at, 0, 0);
+                    const kv8_v4u x = __builtin_amdgcn_raw_buffer_load_b128(vb, at, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 4; i++) vr[t][r][i] = x[i];
                 }
             }
-    };
-    uint32_t c = begin + wave * S::CK;
-    auto advance = [&]() {
-#pragma unroll
-        for (int t = 0; t < S::TILES; t++) {
-            cnv[t] = nv[t];
-            const float k = ks[t] < INFINITY ? ks[t] : 0.0f;      // NaN: 0 by fmaxf
-            cks[t] = fminf(fmaxf(k * g.scale2, 1e-30f), 3.402823466e38f);
-            cvs[t] = vs[t] > 0.0f && vs[t] < INFINITY ? vs[t] : 0.0f;
         }
-        find(c + turn);
     };
-    find(c);
+    uint32_t c = begin + wave * S::CK, n;
+    x = walk.tile(c, walk.page(c));
+    ahead = walk.page(c + turn);
     load_k();
     load_v();
-    advance();
+    walk.scales(x, nks, nvs);
+    // The chunk at c becomes the current one, what the next ones need is read.
+    auto advance = [&]() {
+        walk.settle(nks, nvs, ks, vs);
+        n = x.n;
+        x = walk.tile(c + turn, ahead);
+        walk.scales(x, nks, nvs);
+        ahead = walk.page(c + 2u * turn);
+    };
     while (c < end) {
-        float s[S::TILES][4];
+        advance();
+        float s[1][S::TILES][4];
 #pragma unroll
         for (int t = 0; t < S::TILES; t++) {
             ta_v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -538,16 +595,13 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[t][r] = x[r];
+            for (int r = 0; r < 4; r++) s[0][t][r] = x[r];
         }
         load_k();
-        bool whole = c + S::CK <= sq.past;
-#pragma unroll
-        for (int t = 0; t < S::TILES; t++) whole = whole && cnv[t] == 16u;
-        if (!whole) {
+        if (c + S::CK > sq.past || __any(n != 16u)) {
             // The nodes' chunk, the last, one with a bad page: unseen positions score
             // -inf, and a node's values that are NaN become zeros.
-            kv8_hide(s, (kv8_sees(a, words, node, sq.past, c) & kv8_there(cnv)) >> (4u * lk));
+            kv8_hide(s[0], (kv8_sees(a, words, node, sq.past, c) & kv8_there<S::TILES>(n)) >> (4u * lk));
             if constexpr (F == KV_E4M3)
 #pragma unroll
                 for (int t = 0; t < S::TILES; t++)
@@ -555,11 +609,14 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                     for (int r = 0; r < 4; r++)
 #pragma unroll
                         for (int d = 0; d < S::VD; d++)
-                            vr[t][r][d] = c + 16u * t + 4u * lk + r < sq.past
-                                              ? vr[t][r][d] : kv8_no_nan(vr[t][r][d]);
+                            vr[t][r][d] = kv8_no_nan(
+                                vr[t][r][d], c + 16u * t + 4u * lk + r < sq.past ? 0u : 0x80808080u);
         }
         uint32_t w[S::TILES / 2][S::PN][4];
-        kv8_weigh<T, S::TILES, S::VE>(s, cks, cvs, m, l, o, w);
+        kv8_refer(s, ks, m, l, o);
+#pragma unroll
+        for (int t = 0; t < S::TILES; t++)
+            kv8_weigh(s[0][t], ks[t], vs[t], m[0], l[0], w[t / 2], t % 2);
         // Values: four keys' bytes of one dimension side by side, then widened.
 #pragma unroll
         for (int u = 0; u < S::TILES / 2; u++)
@@ -579,19 +636,18 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                     kv8_bf16<F>(y[1][e], va[2], va[3]);
 #pragma unroll
                     for (int n = S::PN - 1; n >= 0; n--)
-                        o[4 * d + e] = ta_mfma<__bf16>(va, w[u][n], o[4 * d + e]);
+                        o[0][4 * d + e] = ta_mfma<__bf16>(va, w[u][n], o[0][4 * d + e]);
                 }
             }
         load_v();
         c += turn;
-        advance();
     }
 
     // The waves' sums meet, half of the dimensions at a time. Lane's dimensions:
     // VE (4 lk + r) + e.
-    const float sum = lane_sum4(l);
+    const float sum = lane_sum4(l[0]);
     if (lk == 0) {
-        lmax[wave][lm] = m;
+        lmax[wave][lm] = m[0];
         lsum[wave][lm] = sum;
     }
     auto place = [&](uint32_t w, uint32_t col, uint32_t d) {
@@ -606,7 +662,7 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
 #pragma unroll
                 for (int e = 0; e < S::VE; e += 4)
                     *(float4 *)place(wave, lm, S::VE * (4u * lk + r) + e) =
-                        float4{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
+                        float4{o[0][e][r], o[0][e + 1][r], o[0][e + 2][r], o[0][e + 3][r]};
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < 2u * HD; i += 64u * S::W) {
             const uint32_t col = i / (HD / 8u), d = i % (HD / 8u) * 4u + h * (HD / 2u);
@@ -649,10 +705,11 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
 //
 // A prompt's rows: the workgroup's waves share a chunk of CK keys, each with 16 NT
 // rows of its own. Every code is widened once a workgroup: a chunk's codes come into registers
-// while the one before is computed, and leave for the LDS as bf16 (keys of f16 calls
-// f16), the values turned so that a lane reads eight keys of one dimension. Two
-// buffers, one barrier a chunk. Places in the LDS are 16-byte pieces, swapped so that
-// the eight lanes of an access meet no bank twice.
+// while one before is computed, and leave for the LDS as bf16 (keys of f16 calls f16),
+// the values turned so that a lane reads eight keys of one dimension. Keys are a
+// chunk ahead of values, so that the products of the next chunk's scores stand beside
+// this one's exponentials. Two buffers of each, one barrier a chunk. Places in the LDS are 16-byte pieces, swapped so that
+// 16 lanes of an access meet no bank twice.
 template <class T, int HD>
 struct Kv8Wide {
     using S = Kv8Shape<T, HD>;
@@ -663,6 +720,7 @@ struct Kv8Wide {
     static constexpr int KS = HD / 32;              // steps of a score's product
     static constexpr int LB = HD == 64 ? 8 : 16;    // bytes of a thread's keys
     static constexpr int PR = CK / 8;               // pieces of a dimension's keys
+    static constexpr int AHEAD = S::F16 && HD == 128 ? 2 : 3;
 };
 
 template <class T, int F, int HD>
@@ -743,23 +801,18 @@ MYNAH_DEV void kv8_wide(const Kv8Args &g) {
     // four dimensions from td on.
     const uint32_t tk = threadIdx.x / (HD / Z::LB), tp = threadIdx.x % (HD / Z::LB);
     const uint32_t tv = threadIdx.x / (HD / 4), td = threadIdx.x % (HD / 4) * 4u;
-    const bool has_v = tv < Z::CK / 4;
+    const bool has_v = 64 * Z::W == Z::CK / 4 * HD / 4 || tv < Z::CK / 4;
     const uint32_t sb = (uint32_t)a.slot_stride;
     const uint8_t *kbase = (const uint8_t *)a.k + (size_t)kvh * HD;
     const uint8_t *vbase = (const uint8_t *)a.v + (size_t)kvh * HD;
     uint32_t kc[4], vc[4];
-    // The 16 rows of the tile at position p.
-    auto tile = [&](const uint8_t *base, uint32_t p) {
-        unsigned long long r = 0;
-        uint32_t n = 0;
-        if (p < end && cache_row(a, b, p, r)) n = end - p < 16u ? end - p : 16u;
-        else r = 0;
-        return __builtin_amdgcn_make_buffer_rsrc((void *)(base + r * sb), 0, n * sb, 0x00020000);
-    };
-    auto load = [&](uint32_t c) {
-        const uint32_t k16 = __builtin_amdgcn_readfirstlane(tk & ~15u);
-        const uint32_t v16 = __builtin_amdgcn_readfirstlane(4u * tv & ~15u);
-        const auto kb = tile(kbase, c + k16);
+    const Kv8Walk<TILES> walk(g, b, kvh, end);
+    Kv8Tile x[2];                                  // of the next chunk, and the one after it
+    int32_t ahead;                                 // the page of the third
+    float ks[TILES], vs[TILES], nks[2], nvs[2];    // scales of the current one; of the next two
+    uint32_t rows_now;                             // rows of the current one's tiles
+    auto load_k = [&](const Kv8Tile &x) {
+        const auto kb = walk.buffer(kbase, sb, x, __builtin_amdgcn_readfirstlane(tk / 16u));
         const uint32_t at = __umul24(tk & 15u, sb) + Z::LB * tp;
         if constexpr (Z::LB == 16) {
             const kv8_v4u x = __builtin_amdgcn_raw_buffer_load_b128(kb, at, 0, 0);
@@ -770,19 +823,29 @@ MYNAH_DEV void kv8_wide(const Kv8Args &g) {
             kc[0] = x[0];
             kc[1] = x[1];
         }
-        if (has_v) {
-            const auto vb = tile(vbase, c + v16);
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                vc[r] = __builtin_amdgcn_raw_buffer_load_b32(vb, __umul24((4u * tv & 15u) + r, sb) + td,
-                                                             0, 0);
-        }
     };
-    // Widened into the LDS. Key k's piece p (eight dimensions) lies at place p ^ (k &
-    // 7) of its row; keys 16 t + 4 i .. + 3 of dimension d are half t & 1 of piece
-    // 4 (t / 2) + i of d's row, at place piece ^ turn(d).
-    auto turn = [](uint32_t d) { return Z::PR == 8 ? d & 7u : (d >> 2) & 3u; };
-    auto widen = [&](uint32_t c, int buf) {
+    auto load_v = [&](const Kv8Tile &x) {
+        if (!has_v) return;
+        const auto vb = walk.buffer(vbase, sb, x, __builtin_amdgcn_readfirstlane(tv / 4u));
+        const uint32_t at = __umul24(4u * tv & 15u, sb) + td;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            vc[r] = __builtin_amdgcn_raw_buffer_load_b32(vb, at + r * sb, 0, 0);
+    };
+    // Widened into the LDS. Key k's piece p (eight dimensions) lies at place p ^ swap(k)
+    // of its row; keys 16 t + 4 i .. + 3 of dimension d are half t & 1 of piece 4 (t / 2)
+    // + i of d's row, at place piece ^ turn(d).
+    auto swap = [](uint32_t k) { return HD == 64 ? (k >> 1) & 7u : k & 15u; };
+    auto turn = [](uint32_t d) { return Z::PR == 8 ? (d >> 1) & 7u : (d >> 2) & 3u; };
+    // f16 calls have no registers for where a thread writes, and find it anew each time.
+    auto anew = [](uint32_t v) {
+        if constexpr (S::F16 && HD == 128) asm volatile("" : "+v"(v));
+        return v;
+    };
+    auto widen_k = [&](int buf) {
+        // Piece LB / 8 tp of key tk.
+        const uint32_t i = anew(threadIdx.x), tk = i / (HD / Z::LB), tp = i % (HD / Z::LB);
+        const uint32_t to = tk * (HD / 8) + ((Z::LB / 8 * tp) ^ swap(tk));
 #pragma unroll
         for (int p = 0; p < Z::LB / 8; p++) {
             uint4 w;
@@ -793,119 +856,145 @@ MYNAH_DEV void kv8_wide(const Kv8Args &g) {
                 kv8_bf16<F>(kc[2 * p], w.x, w.y);
                 kv8_bf16<F>(kc[2 * p + 1], w.z, w.w);
             }
-            kl[buf][tk * (HD / 8) + ((Z::LB / 8 * tp + p) ^ (tk & 7u))] = w;
+            kl[buf][to ^ p] = w;                   // LB / 8 tp is even where p is not 0 alone
         }
-        if (has_v) {
-            if constexpr (F == KV_E4M3)
+    };
+    auto widen_v = [&](uint32_t c, int buf) {
+        if (!has_v) return;
+        // td's half piece, in halves (turn(td + 2) is turn(td) ^ 1 for eight pieces a
+        // row, and turn(td) for four).
+        const uint32_t id = anew(threadIdx.x), tv = id / (HD / 4), td = id % (HD / 4) * 4u;
+        const uint32_t to = 2u * (td * Z::PR + ((tv / 8u * 4u + (tv & 3u)) ^ turn(td))) + (tv / 4u & 1u);
+        uint32_t y[4];
+        kv8_turn(vc, y);
+        if constexpr (F == KV_E4M3) {              // a node's NaN is 0
+            const uint32_t p = c + 4u * tv, old = sq.past > p ? sq.past - p : 0u;
+            const uint32_t nodes = old < 4u ? 0x80808080u << (8u * old) : 0u;
 #pragma unroll
-                for (int r = 0; r < 4; r++)        // a node's NaN is 0
-                    vc[r] = c + 4u * tv + r < sq.past ? vc[r] : kv8_no_nan(vc[r]);
-            uint32_t y[4];
-            kv8_turn(vc, y);
-            const uint32_t t = tv / 4u, piece = t / 2u * 4u + (tv & 3u);
+            for (int i = 0; i < 4; i++) y[i] = kv8_no_nan(y[i], nodes);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint2 w;
-                kv8_bf16<F>(y[i], w.x, w.y);
-                const uint32_t d = td + i;
-                *((uint2 *)&vl[buf][d * Z::PR + (piece ^ turn(d))] + (t & 1u)) = w;
-            }
+        for (int i = 0; i < 4; i++) {
+            uint2 w;
+            kv8_bf16<F>(y[i], w.x, w.y);
+            ((uint2 *)vl[buf])[(Z::PR == 8 ? to ^ (i & 2) : to) + 2 * i * Z::PR] = w;
         }
     };
 
-    float ks[TILES], vs[TILES];
-    uint32_t cnv[TILES];
-    auto scales = [&](uint32_t c) {
-#pragma unroll
-        for (int t = 0; t < TILES; t++) {
-            const uint32_t p = c + 16u * t;
-            unsigned long long r;
-            cnv[t] = 0;
-            ks[t] = vs[t] = 0.0f;
-            if (p >= end || !cache_row(a, b, p, r)) continue;
-            cnv[t] = end - p < 16u ? end - p : 16u;
-            const size_t at = (size_t)(r >> g.block_log2) * a.n_kv + kvh;
-            const float k = scalar_f32(g.ks, at), v = scalar_f32(g.vs, at);
-            ks[t] = k < INFINITY ? k : 0.0f;
-            vs[t] = v > 0.0f && v < INFINITY ? v : 0.0f;
-        }
-#pragma unroll
-        for (int t = 0; t < TILES; t++)
-            ks[t] = fminf(fmaxf(ks[t] * g.scale2, 1e-30f), 3.402823466e38f);
-    };
     // The lane's places: of piece 4 k + lk of key lm, and of 4 u + lk of dimension lm.
-    const uint32_t kat[2] = {lm * (HD / 8) + (lk ^ (lm & 7u)), lm * (HD / 8) + ((4u + lk) ^ (lm & 7u))};
+    constexpr int KA = HD == 64 ? 2 : 4;
+    uint32_t kat[KA];
+#pragma unroll
+    for (int k = 0; k < KA; k++) kat[k] = lm * (HD / 8) + ((4u * k + lk) ^ swap(lm));
     uint32_t vat[TILES / 2];
 #pragma unroll
     for (int u = 0; u < TILES / 2; u++) vat[u] = lm * Z::PR + ((4u * u + lk) ^ turn(lm));
-    auto compute = [&](uint32_t c, int buf) {
-        float s[NT][TILES][4];
-#pragma unroll
-        for (int t = 0; t < TILES; t++) {
-            ta_v4f x[NT];
-#pragma unroll
-            for (int n = 0; n < NT; n++) x[n] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < Z::KS; k++) {
-                const uint4 kk = kl[buf][kat[k % 2] + 16 * t * (HD / 8) + 8 * (k / 2)];
-                const uint32_t w[4] = {kk.x, kk.y, kk.z, kk.w};
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int i = S::QN - 1; i >= 0; i--) {
-                        if constexpr (S::F16) x[n] = ta_mfma<_Float16>(w, qv[n][i][k], x[n]);
-                        else x[n] = ta_mfma<__bf16>(w, qv[n][i][k], x[n]);
-                    }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) s[n][t][r] = x[n][r];
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        bool whole = c + Z::CK <= sq.past + (chain ? first_node : 0u);
-#pragma unroll
-        for (int t = 0; t < TILES; t++) whole = whole && cnv[t] == 16u;
-        if (!whole) {
-            const uint64_t there = kv8_there(cnv);
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-                kv8_hide(s[n], (kv8_sees(a, lwords[wave][16 * n + lm], lnode[wave][16 * n + lm],
-                                         sq.past, c) & there) >> (4u * lk));
-        }
-        uint32_t w[NT][TILES / 2][S::PN][4];
+    float s[2][NT][TILES][4];
+    constexpr int SQ = TILES * Z::KS, SV = TILES / 2 * S::VE;  // steps of the two products
+    auto key = [&](int buf, int i) {                           // a step's operands
+        return kl[buf][kat[i % Z::KS % KA] + 16 * (i / Z::KS) * (HD / 8) + 4 * KA * (i % Z::KS / KA)];
+    };
+    auto value = [&](int buf, int i) { return vl[buf][vat[i / S::VE] + 16 * (i % S::VE) * Z::PR]; };
+    // Step i of a chunk's scores: tile i / KS, dimensions 32 (i % KS) ..
+    auto score = [&](float (&to)[NT][TILES][4], const uint4 &kk, int i) {
+        const uint32_t w[4] = {kk.x, kk.y, kk.z, kk.w};
+        const int t = i / Z::KS, k = i % Z::KS;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            kv8_weigh<T, TILES, S::VE>(s[n], ks, vs, m[n], l[n], o[n], w[n]);
+            ta_v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (k)
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[r] = to[n][t][r];
+#pragma unroll
+            for (int j = S::QN - 1; j >= 0; j--) {
+                if constexpr (S::F16) x = ta_mfma<_Float16>(w, qv[n][j][k], x);
+                else x = ta_mfma<__bf16>(w, qv[n][j][k], x);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) to[n][t][r] = x[r];
+        }
+    };
+    // Chunk c, whose scores are s[buf] and whose values are in buffer `buf`. The scores
+    // of the next one, whose keys are in the other, are made beside its exponentials,
+    // and the codes that have come are widened beside its second product, step by
+    // step: the compiler by itself puts all products behind all else. Operands are
+    // read AHEAD steps ahead.
+    constexpr int AHEAD = Z::AHEAD, RING = AHEAD + 1;
+    auto compute = [&](uint32_t c, int buf) {
+        if (c + Z::CK > sq.past + (chain ? first_node : 0u) || __any(rows_now != 16u)) {
+            const uint64_t there = kv8_there<TILES>(rows_now);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                kv8_hide(s[buf][n], (kv8_sees(a, lwords[wave][16 * n + lm], lnode[wave][16 * n + lm],
+                                              sq.past, c) & there) >> (4u * lk));
+        }
+        uint4 op[RING];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) op[i] = key(1 - buf, i);
+        kv8_refer(s[buf], ks, m, l, o);
+        uint32_t w[NT][TILES / 2][S::PN][4];
+        constexpr int G = NT * TILES;              // tiles of all columns
+#pragma unroll
+        for (int i = 0; i < SQ; i++) {
+            op[(i + AHEAD) % RING] = i + AHEAD < SQ ? key(1 - buf, i + AHEAD) : value(buf, i + AHEAD - SQ);
+            score(s[1 - buf], op[i % RING], i);
+#pragma unroll
+            for (int j = i * G / SQ; j < (i + 1) * G / SQ; j++)
+                kv8_weigh(s[buf][j % NT][j / NT], ks[j / NT], vs[j / NT], m[j % NT], l[j % NT],
+                          w[j % NT][j / NT / 2], j / NT % 2);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int u = 0; u < TILES / 2; u++)
+        for (int i = 0; i < SV; i++) {
+            const int at = SQ + i;
+            if (i + AHEAD < SV) op[(at + AHEAD) % RING] = value(buf, i + AHEAD);
+            const uint4 vv = op[at % RING];
+            const uint32_t va[4] = {vv.x, vv.y, vv.z, vv.w};
 #pragma unroll
-            for (int e = 0; e < S::VE; e++) {
-                const uint4 vv = vl[buf][vat[u] + 16 * e * Z::PR];
-                const uint32_t va[4] = {vv.x, vv.y, vv.z, vv.w};
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int i = S::PN - 1; i >= 0; i--)
-                        o[n][e] = ta_mfma<__bf16>(va, w[n][u][i], o[n][e]);
-            }
-        __builtin_amdgcn_sched_barrier(0);
+                for (int j = S::PN - 1; j >= 0; j--)
+                    o[n][i % S::VE] = ta_mfma<__bf16>(va, w[n][i / S::VE][j], o[n][i % S::VE]);
+            if (i == SV / 4) widen_k(buf);
+            if (i == SV / 2) widen_v(c + Z::CK, 1 - buf);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
-    load(begin);
-    widen(begin, 0);
+    x[0] = walk.tile(begin, walk.page(begin));
+    x[1] = walk.tile(begin + Z::CK, walk.page(begin + Z::CK));
+    ahead = walk.page(begin + 2u * Z::CK);
+    load_k(x[0]);
+    load_v(x[0]);
+    walk.scales(x[0], nks[0], nvs[0]);
+    walk.scales(x[1], nks[1], nvs[1]);
+    widen_k(0);
+    load_k(x[1]);
+    widen_v(begin, 0);
+    widen_k(1);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SQ; i++) score(s[0], key(0, i), i);
     __syncthreads();
     for (uint32_t c = begin; c < end; c += 2u * Z::CK) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint32_t at = c + h * Z::CK;
-            load(at + Z::CK);
+            load_v(x[1]);
+            walk.settle(nks[0], nvs[0], ks, vs);
+            rows_now = x[0].n;
+            x[0] = x[1];
+            x[1] = walk.tile(at + 2u * Z::CK, ahead);
+            load_k(x[1]);
+            nks[0] = nks[1];
+            nvs[0] = nvs[1];
+            walk.scales(x[1], nks[1], nvs[1]);
+            ahead = walk.page(at + 3u * Z::CK);
             if (at < mine) {
-                scales(at);
                 compute(at, h);
+            } else {
+                widen_k(h);
+                widen_v(at + Z::CK, 1 - h);
             }
-            widen(at + Z::CK, 1 - h);
             __syncthreads();
         }
     }
