@@ -125,26 +125,39 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *p, void *stream) {
 
 /* ── attention ───────────────────────────────────────────────────────────── */
 
-/* What a call launches: kernel family `wide` or not, a workgroup of 8 waves for each
- * key head, group of `rows` query rows and slot: a sequence's, or with more slots
- * than sequences a piece of one. */
+/* What a call launches: kernels of few rows (16 `tiles` a workgroup) or, wide,
+ * of many; a workgroup of `waves` waves for each key head, group of `rows` query rows
+ * and slot: a sequence's, or with more slots than sequences a piece of one. */
 typedef struct {
-    uint32_t wide, rows, groups, slots;
+    uint32_t wide, tiles, waves, rows, groups, slots;
 } kv8_plan;
-#define KV8_WAVES 8u
+#define KV8_WAVES 4u                /* of the kernels of few rows (= Kv8Shape::W) */
+#define KV8_WIDE_WAVES 8u           /* of those of many (= Kv8Wide::W) */
 
 static void make_plan(const mynah_kv8_attention *p, uint32_t cus, kv8_plan *t) {
-    const uint32_t group = p->n_heads / p->cache.n_kv_heads;
+    const uint32_t group = p->n_heads / p->cache.n_kv_heads, hd = p->cache.head_dim;
     const uint64_t rows = (uint64_t)p->max_nodes * group;
-    t->wide = rows > 64u;
-    t->rows = !t->wide ? 16u : p->type == MYNAH_F32 || p->cache.head_dim == 256 ? 128u : 256u;
+    /* From 33 rows on the shared chunk wins: four sequences of 16 nodes over 4000
+     * positions (bf16, 32 heads, 8 of keys, 64 rows a key head) 30 us for 38, of 32
+     * nodes over 8000 47 for 62; 96 rows of one sequence of 4000 24 both ways. */
+    t->wide = rows > 32;
+    t->tiles = rows > 16 && hd != 256 ? 2u : 1u;
+    t->waves = t->wide ? KV8_WIDE_WAVES : KV8_WAVES;
+    t->rows = !t->wide ? 16u * t->tiles : p->type == MYNAH_F32 || hd == 256 ? 128u : 256u;
     t->groups = (uint32_t)((rows + t->rows - 1) / t->rows);
     const uint64_t base = (uint64_t)p->cache.n_kv_heads * t->groups;
-    const uint32_t chunk = p->cache.head_dim == 256 ? 32u : 64u;
+    const uint32_t chunk = t->wide ? (hd == 256 ? 32u : 64u) : hd * t->tiles >= 256 ? 32u : 64u;
     const uint32_t turn = t->wide ? chunk : KV8_WAVES * chunk;
-    const uint64_t turns = (uint64_t)p->n_seqs * ((p->max_kv + turn - 1) / turn);
-    uint64_t s = cus / base;
-    if (s > turns) s = turns;
+    /* Pieces enough for every CU, of a turn each at least; and, of 16 turns at least,
+     * four workgroups a CU, so that long sequences beside short ones do not set the
+     * time alone: 32 of up to 16,384 e4m3 positions 134 us, 144 with two, 186 with one. A
+     * sequence cut in two costs 4 to 5 us of a join and as much again in the workgroups: 32
+     * of 4000 positions 46 us uncut, 58 cut, 64 of up to 2048 36 and 46. */
+    const uint64_t turns = (p->max_kv + turn - 1) / turn;
+    uint64_t s = cus / base, more = 4 * cus / base;
+    if (s > p->n_seqs * turns) s = p->n_seqs * turns;
+    if (more > p->n_seqs * ((turns + 15) / 16)) more = p->n_seqs * ((turns + 15) / 16);
+    if (!t->wide && s < more) s = more;
     if (s > 256) s = 256;                       /* four sequences a lane share them */
     t->slots = s > p->n_seqs ? (uint32_t)s : p->n_seqs;
 }
@@ -183,7 +196,7 @@ static int attn_check(const mynah_kv8_attention *p) {
     if (!isfinite(p->scale)) return refuse("kv8_attention: the scale must be finite");
     kv8_plan t;                                 /* of whole sequences, the most there are */
     make_plan(p, 1, &t);
-    if ((uint64_t)p->n_seqs * c->n_kv_heads * t.groups > MYNAH_MOST_WGS(64 * KV8_WAVES))
+    if ((uint64_t)p->n_seqs * c->n_kv_heads * t.groups > MYNAH_MOST_WGS(64 * t.waves))
         return refuse("kv8_attention: too many workgroups for one launch");
     return 0;
 }
@@ -263,8 +276,9 @@ int mynah_hip_kv8_attention_dev(const mynah_kv8_attention *p, void *workspace,
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a}, *join[] = {&a.t};
     const int h = c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2, ti = type_index(p->type);
-    if (mynah_launch(d, (t.wide ? MYNAH_K_KV8_WIDE : MYNAH_K_KV8_ATTN) + 6 * ti + 2 * h + c->format, (unsigned)wgs, 1,
-                     64 * KV8_WAVES, 0, st, args) != 0)
+    if (mynah_launch(d, t.wide ? MYNAH_K_KV8_WIDE + 6 * ti + 2 * h + c->format
+                               : MYNAH_K_KV8_ATTN + 10 * ti + 5 * c->format + 2 * h + (int)t.tiles - 1, (unsigned)wgs, 1,
+                     64 * t.waves, 0, st, args) != 0)
         return -1;
     if (t.slots == p->n_seqs) return 0;
     return mynah_launch3(d, MYNAH_K_TREE_JOIN + 3 * ti + h, p->n_seqs, p->max_nodes,

@@ -254,17 +254,17 @@ MYNAH_DEV uint32_t kv8_no_nan(uint32_t d, uint32_t which) {
     return d & ~(n - (n >> 7));
 }
 
-template <class T, int HD>
+template <class T, int HD, int NT = 1>
 struct Kv8Shape {
     static constexpr bool F32 = sizeof(T) == 4, F16 = __is_same(T, _Float16);
     static constexpr int QN = F32 ? 3 : 1;              // numbers that a query value is
     static constexpr int PN = F32 ? 3 : F16 ? 2 : 1;    // ... that a weight is
-    static constexpr int TILES = HD == 256 ? 2 : 4;     // 16-key tiles of a chunk
+    static constexpr int TILES = HD * NT >= 256 ? 2 : 4; // 16-key tiles of a chunk
     static constexpr int CK = 16 * TILES;
     static constexpr int KP = HD / 64;                  // 16-byte pieces of a lane's key
     static constexpr int VE = HD / 16;                  // dimensions (O tiles) of a lane
     static constexpr int VD = HD / 64;                  // dwords of a lane's value row
-    static constexpr int W = 8;
+    static constexpr int W = 4;                         // (= KV8_WAVES in kv8.c)
 };
 
 // Two f32 numbers cut to bf16, and what is left of them.
@@ -462,14 +462,14 @@ struct Kv8Walk {
     }
 };
 
-// A workgroup's W waves take chunks of CK keys in turn, for the same 16 queries,
+// A workgroup's W waves take chunks of CK keys in turn, for the same 16 NT queries,
 // straight from memory into registers: a chunk's keys are under way while the one
 // before is weighed, its values while its scores are made. The waves' results meet
-// at the end. Grid slots * n_kv * groups (of 16 query rows), block 64 W; the order
+// at the end. Grid slots * n_kv * groups (of 16 NT query rows), block 64 W; the order
 // of workgroups as in tree_attn.
-template <class T, int F, int HD>
+template <class T, int F, int HD, int NT>
 MYNAH_DEV void kv8_attn(const Kv8Args &g) {
-    using S = Kv8Shape<T, HD>;
+    using S = Kv8Shape<T, HD, NT>;
     const TreeArgs &a = g.t;
     __shared__ __attribute__((aligned(16))) float part[S::W * 16 * HD / 2];
     __shared__ float lmax[S::W][16], lsum[S::W][16];
@@ -489,7 +489,7 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
     const uint32_t b = __builtin_amdgcn_readfirstlane(share.b);
     const uint32_t split = __builtin_amdgcn_readfirstlane(share.split);
     const SeqSpan sq = seq_span(a, b);
-    const uint32_t rows = sq.nodes * a.group, wg0 = grp * 16u;
+    const uint32_t rows = sq.nodes * a.group, wg0 = grp * (16u * NT);
     if (wg0 >= rows) return;                       // uniform
     uint32_t per = __builtin_amdgcn_readfirstlane(share.per);
     if (per == 0u) {
@@ -500,22 +500,29 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
     const uint32_t begin = from < sq.kv ? (uint32_t)from : sq.kv;
     const uint32_t end = sq.kv - begin < per ? sq.kv : begin + per;
 
-    // The lane's query as operands: piece h of 16 dimensions is 16 (lk + 4 h) ..,
+    // The lane's queries as operands: piece h of 16 dimensions is 16 (lk + 4 h) ..,
     // half j of it one step of the product.
-    const uint32_t rr = wg0 + lm, node = rr / a.group;
-    const long long qrow = sq.row0 + node;
-    const bool live = rr < rows && qrow >= 0 && qrow < (long long)a.n_rows;
-    const size_t words = live ? (size_t)qrow * a.mask_words : 0;
-    uint32_t qv[S::QN][2 * S::KP][4];
-    const T *q = (const T *)a.q + (live ? (size_t)qrow * a.q_stride : 0) +
-                 (size_t)(kvh * a.group + rr - node * a.group) * HD;
+    uint32_t node[NT], qv[NT][S::QN][2 * S::KP][4];
+    size_t words[NT];
+    float m[NT], l[NT];
+    ta_v4f o[NT][S::VE];
 #pragma unroll
-    for (int k = 0; k < 2 * S::KP; k++)
-        kv8_query<T>(q + 16u * (lk + 4u * (k / 2)) + 8u * (k % 2), live, a.flip, qv, k);
-    float m[1] = {-INFINITY}, l[1] = {0.0f};
-    ta_v4f o[1][S::VE];
+    for (int j = 0; j < NT; j++) {
+        const uint32_t rr = wg0 + 16u * j + lm;
+        node[j] = rr / a.group;
+        const long long qrow = sq.row0 + node[j];
+        const bool live = rr < rows && qrow >= 0 && qrow < (long long)a.n_rows;
+        words[j] = live ? (size_t)qrow * a.mask_words : 0;
+        const T *q = (const T *)a.q + (live ? (size_t)qrow * a.q_stride : 0) +
+                     (size_t)(kvh * a.group + rr - node[j] * a.group) * HD;
 #pragma unroll
-    for (int e = 0; e < S::VE; e++) o[0][e] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < 2 * S::KP; k++)
+            kv8_query<T>(q + 16u * (lk + 4u * (k / 2)) + 8u * (k % 2), live, a.flip, qv[j], k);
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < S::VE; e++) o[j][e] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     const uint32_t sb = (uint32_t)a.slot_stride;
     const uint8_t *kbase = (const uint8_t *)a.k + (size_t)kvh * HD;
@@ -575,10 +582,12 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
     };
     while (c < end) {
         advance();
-        float s[1][S::TILES][4];
+        float s[NT][S::TILES][4];
 #pragma unroll
         for (int t = 0; t < S::TILES; t++) {
-            ta_v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+            ta_v4f acc[NT];
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[j] = ta_v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int k = 0; k < 2 * S::KP; k++) {
                 uint32_t w[4];
@@ -589,19 +598,26 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                     else kv8_bf16<F>(d, w[2 * i], w[2 * i + 1]);
                 }
 #pragma unroll
-                for (int n = S::QN - 1; n >= 0; n--) {
-                    if constexpr (S::F16) x = ta_mfma<_Float16>(w, qv[n][k], x);
-                    else x = ta_mfma<__bf16>(w, qv[n][k], x);
-                }
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int i = S::QN - 1; i >= 0; i--) {
+                        if constexpr (S::F16) acc[j] = ta_mfma<_Float16>(w, qv[j][i][k], acc[j]);
+                        else acc[j] = ta_mfma<__bf16>(w, qv[j][i][k], acc[j]);
+                    }
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[0][t][r] = x[r];
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[j][t][r] = acc[j][r];
         }
         load_k();
         if (c + S::CK > sq.past || __any(n != 16u)) {
             // The nodes' chunk, the last, one with a bad page: unseen positions score
             // -inf, and a node's values that are NaN become zeros.
-            kv8_hide(s[0], (kv8_sees(a, words, node, sq.past, c) & kv8_there<S::TILES>(n)) >> (4u * lk));
+            const uint64_t there = kv8_there<S::TILES>(n);
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                kv8_hide(s[j], (kv8_sees(a, words[j], node[j], sq.past, c) & there) >> (4u * lk));
             if constexpr (F == KV_E4M3)
 #pragma unroll
                 for (int t = 0; t < S::TILES; t++)
@@ -612,11 +628,13 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                             vr[t][r][d] = kv8_no_nan(
                                 vr[t][r][d], c + 16u * t + 4u * lk + r < sq.past ? 0u : 0x80808080u);
         }
-        uint32_t w[S::TILES / 2][S::PN][4];
+        uint32_t w[NT][S::TILES / 2][S::PN][4];
         kv8_refer(s, ks, m, l, o);
 #pragma unroll
-        for (int t = 0; t < S::TILES; t++)
-            kv8_weigh(s[0][t], ks[t], vs[t], m[0], l[0], w[t / 2], t % 2);
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int t = 0; t < S::TILES; t++)
+                kv8_weigh(s[j][t], ks[t], vs[t], m[j], l[j], w[j][t / 2], t % 2);
         // Values: four keys' bytes of one dimension side by side, then widened.
 #pragma unroll
         for (int u = 0; u < S::TILES / 2; u++)
@@ -635,38 +653,44 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                     kv8_bf16<F>(y[0][e], va[0], va[1]);
                     kv8_bf16<F>(y[1][e], va[2], va[3]);
 #pragma unroll
-                    for (int n = S::PN - 1; n >= 0; n--)
-                        o[0][4 * d + e] = ta_mfma<__bf16>(va, w[u][n], o[0][4 * d + e]);
+                    for (int j = 0; j < NT; j++)
+#pragma unroll
+                        for (int i = S::PN - 1; i >= 0; i--)
+                            o[j][4 * d + e] = ta_mfma<__bf16>(va, w[j][u][i], o[j][4 * d + e]);
                 }
             }
         load_v();
         c += turn;
     }
 
-    // The waves' sums meet, half of the dimensions at a time. Lane's dimensions:
-    // VE (4 lk + r) + e.
-    const float sum = lane_sum4(l[0]);
-    if (lk == 0) {
-        lmax[wave][lm] = m[0];
-        lsum[wave][lm] = sum;
-    }
+    // The waves' sums meet, a column tile and half of the dimensions at a time. Lane's
+    // dimensions: VE (4 lk + r) + e.
     auto place = [&](uint32_t w, uint32_t col, uint32_t d) {
         return part + (16u * w + col) * (HD / 2) + 4u * ((d % (HD / 2) / 4u) ^ (col & 7u));
     };
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int h = 0; h < 2 * NT; h++) {
+        constexpr int HALF = HD / 2;
+        const int j = h / 2;
         __syncthreads();
-        if (lk / 2u == (uint32_t)h)
+        if (h % 2 == 0) {
+            const float sum = lane_sum4(l[j]);
+            if (lk == 0) {
+                lmax[wave][lm] = m[j];
+                lsum[wave][lm] = sum;
+            }
+        }
+        if (lk / 2u == (uint32_t)(h % 2))
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int e = 0; e < S::VE; e += 4)
                     *(float4 *)place(wave, lm, S::VE * (4u * lk + r) + e) =
-                        float4{o[0][e][r], o[0][e + 1][r], o[0][e + 2][r], o[0][e + 3][r]};
+                        float4{o[j][e][r], o[j][e + 1][r], o[j][e + 2][r], o[j][e + 3][r]};
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < 2u * HD; i += 64u * S::W) {
-            const uint32_t col = i / (HD / 8u), d = i % (HD / 8u) * 4u + h * (HD / 2u);
-            const uint32_t r = wg0 + col, nd = r / a.group;
+            const uint32_t col = i / (HD / 8u), d = i % (HD / 8u) * 4u + h % 2 * HALF;
+            const uint32_t r = wg0 + 16u * j + col, nd = r / a.group;
             const long long orow = sq.row0 + nd;
             if (r >= rows || orow < 0 || orow >= (long long)a.n_rows) continue;
             float best = -INFINITY, all = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -684,7 +708,7 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
                 v[3] = fmaf(f, x.w, v[3]);
             }
             if (a.slots > a.n_seqs) {
-                const size_t at = (size_t)id * 16u + col;
+                const size_t at = (size_t)id * (16u * NT) + 16u * j + col;
                 if (d == 0u) {
                     a.pm[at] = best;
                     a.pl[at] = all;
@@ -1027,19 +1051,21 @@ MYNAH_DEV void kv8_wide(const Kv8Args &g) {
     }
 }
 
-#define KV8_ATTN(name, T, fmt, F, HD)                                                        \
-    extern "C" __global__ void __launch_bounds__((64 * Kv8Shape<T, HD>::W), 2)               \
-        mynah_kv8_attn_##name##_##fmt##_##HD(Kv8Args a) { kv8_attn<T, F, HD>(a); }           \
+#define KV8_ATTN(name, T, fmt, F, HD, NT, WAVES)                                             \
+    extern "C" __global__ void __launch_bounds__((64 * Kv8Shape<T, HD, NT>::W), WAVES)       \
+        mynah_kv8_attn_##name##_##fmt##_##HD##_##NT(Kv8Args a) { kv8_attn<T, F, HD, NT>(a); }
+#define KV8_WIDE(name, T, fmt, F, HD)                                                        \
     extern "C" __global__ void __launch_bounds__((64 * Kv8Wide<T, HD>::W), 2)                \
         mynah_kv8_wide_##name##_##fmt##_##HD(Kv8Args a) { kv8_wide<T, F, HD>(a); }
-#define KV8_ATTNS(name, T, HD) \
-    KV8_ATTN(name, T, i8, KV_I8, HD) KV8_ATTN(name, T, e4m3, KV_E4M3, HD)
-KV8_ATTNS(f32, float, 64)
-KV8_ATTNS(f32, float, 128)
-KV8_ATTNS(f32, float, 256)
-KV8_ATTNS(f16, _Float16, 64)
-KV8_ATTNS(f16, _Float16, 128)
-KV8_ATTNS(f16, _Float16, 256)
-KV8_ATTNS(bf16, __bf16, 64)
-KV8_ATTNS(bf16, __bf16, 128)
-KV8_ATTNS(bf16, __bf16, 256)
+// Two waves a SIMD; one of f32 queries of 256 values, which take 96 registers.
+#define KV8_ATTNS(name, T, fmt, F)                                              \
+    KV8_ATTN(name, T, fmt, F, 64, 1, 2) KV8_ATTN(name, T, fmt, F, 64, 2, 2)     \
+    KV8_ATTN(name, T, fmt, F, 128, 1, 2) KV8_ATTN(name, T, fmt, F, 128, 2, 2)   \
+    KV8_ATTN(name, T, fmt, F, 256, 1, (sizeof(T) == 4 ? 1 : 2))                 \
+    KV8_WIDE(name, T, fmt, F, 64) KV8_WIDE(name, T, fmt, F, 128) KV8_WIDE(name, T, fmt, F, 256)
+KV8_ATTNS(f32, float, i8, KV_I8)
+KV8_ATTNS(f32, float, e4m3, KV_E4M3)
+KV8_ATTNS(f16, _Float16, i8, KV_I8)
+KV8_ATTNS(f16, _Float16, e4m3, KV_E4M3)
+KV8_ATTNS(bf16, __bf16, i8, KV_I8)
+KV8_ATTNS(bf16, __bf16, e4m3, KV_E4M3)

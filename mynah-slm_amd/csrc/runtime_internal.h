@@ -211,24 +211,36 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_KV8_STORE_BF16_128_4, "mynah_kv8_store_bf16_128_4") \
     X(MYNAH_K_KV8_STORE_BF16_256_1, "mynah_kv8_store_bf16_256_1") \
     X(MYNAH_K_KV8_STORE_BF16_256_4, "mynah_kv8_store_bf16_256_4") \
-    X(MYNAH_K_KV8_ATTN, "mynah_kv8_attn_f32_i8_64") \
-    X(MYNAH_K_KV8_ATTN_F32_E4M3_64, "mynah_kv8_attn_f32_e4m3_64") \
-    X(MYNAH_K_KV8_ATTN_F32_I8_128, "mynah_kv8_attn_f32_i8_128") \
-    X(MYNAH_K_KV8_ATTN_F32_E4M3_128, "mynah_kv8_attn_f32_e4m3_128") \
-    X(MYNAH_K_KV8_ATTN_F32_I8_256, "mynah_kv8_attn_f32_i8_256") \
-    X(MYNAH_K_KV8_ATTN_F32_E4M3_256, "mynah_kv8_attn_f32_e4m3_256") \
-    X(MYNAH_K_KV8_ATTN_F16_I8_64, "mynah_kv8_attn_f16_i8_64") \
-    X(MYNAH_K_KV8_ATTN_F16_E4M3_64, "mynah_kv8_attn_f16_e4m3_64") \
-    X(MYNAH_K_KV8_ATTN_F16_I8_128, "mynah_kv8_attn_f16_i8_128") \
-    X(MYNAH_K_KV8_ATTN_F16_E4M3_128, "mynah_kv8_attn_f16_e4m3_128") \
-    X(MYNAH_K_KV8_ATTN_F16_I8_256, "mynah_kv8_attn_f16_i8_256") \
-    X(MYNAH_K_KV8_ATTN_F16_E4M3_256, "mynah_kv8_attn_f16_e4m3_256") \
-    X(MYNAH_K_KV8_ATTN_BF16_I8_64, "mynah_kv8_attn_bf16_i8_64") \
-    X(MYNAH_K_KV8_ATTN_BF16_E4M3_64, "mynah_kv8_attn_bf16_e4m3_64") \
-    X(MYNAH_K_KV8_ATTN_BF16_I8_128, "mynah_kv8_attn_bf16_i8_128") \
-    X(MYNAH_K_KV8_ATTN_BF16_E4M3_128, "mynah_kv8_attn_bf16_e4m3_128") \
-    X(MYNAH_K_KV8_ATTN_BF16_I8_256, "mynah_kv8_attn_bf16_i8_256") \
-    X(MYNAH_K_KV8_ATTN_BF16_E4M3_256, "mynah_kv8_attn_bf16_e4m3_256") \
+    X(MYNAH_K_KV8_ATTN, "mynah_kv8_attn_f32_i8_64_1") \
+    X(MYNAH_K_KV8_ATTN_F32_I8_64_2, "mynah_kv8_attn_f32_i8_64_2") \
+    X(MYNAH_K_KV8_ATTN_F32_I8_128_1, "mynah_kv8_attn_f32_i8_128_1") \
+    X(MYNAH_K_KV8_ATTN_F32_I8_128_2, "mynah_kv8_attn_f32_i8_128_2") \
+    X(MYNAH_K_KV8_ATTN_F32_I8_256_1, "mynah_kv8_attn_f32_i8_256_1") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_64_1, "mynah_kv8_attn_f32_e4m3_64_1") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_64_2, "mynah_kv8_attn_f32_e4m3_64_2") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_128_1, "mynah_kv8_attn_f32_e4m3_128_1") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_128_2, "mynah_kv8_attn_f32_e4m3_128_2") \
+    X(MYNAH_K_KV8_ATTN_F32_E4M3_256_1, "mynah_kv8_attn_f32_e4m3_256_1") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_64_1, "mynah_kv8_attn_f16_i8_64_1") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_64_2, "mynah_kv8_attn_f16_i8_64_2") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_128_1, "mynah_kv8_attn_f16_i8_128_1") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_128_2, "mynah_kv8_attn_f16_i8_128_2") \
+    X(MYNAH_K_KV8_ATTN_F16_I8_256_1, "mynah_kv8_attn_f16_i8_256_1") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_64_1, "mynah_kv8_attn_f16_e4m3_64_1") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_64_2, "mynah_kv8_attn_f16_e4m3_64_2") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_128_1, "mynah_kv8_attn_f16_e4m3_128_1") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_128_2, "mynah_kv8_attn_f16_e4m3_128_2") \
+    X(MYNAH_K_KV8_ATTN_F16_E4M3_256_1, "mynah_kv8_attn_f16_e4m3_256_1") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_64_1, "mynah_kv8_attn_bf16_i8_64_1") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_64_2, "mynah_kv8_attn_bf16_i8_64_2") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_128_1, "mynah_kv8_attn_bf16_i8_128_1") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_128_2, "mynah_kv8_attn_bf16_i8_128_2") \
+    X(MYNAH_K_KV8_ATTN_BF16_I8_256_1, "mynah_kv8_attn_bf16_i8_256_1") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_64_1, "mynah_kv8_attn_bf16_e4m3_64_1") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_64_2, "mynah_kv8_attn_bf16_e4m3_64_2") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_128_1, "mynah_kv8_attn_bf16_e4m3_128_1") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_128_2, "mynah_kv8_attn_bf16_e4m3_128_2") \
+    X(MYNAH_K_KV8_ATTN_BF16_E4M3_256_1, "mynah_kv8_attn_bf16_e4m3_256_1") \
     X(MYNAH_K_KV8_WIDE, "mynah_kv8_wide_f32_i8_64") \
     X(MYNAH_K_KV8_WIDE_F32_E4M3_64, "mynah_kv8_wide_f32_e4m3_64") \
     X(MYNAH_K_KV8_WIDE_F32_I8_128, "mynah_kv8_wide_f32_i8_128") \
