@@ -8,6 +8,9 @@
 
 #include <string.h>
 
+/* Entries of a thread where one workgroup forks (= PG_FORK in pages.hip). */
+#define PAGES_FORK 8u
+
 static int pool_check(const mynah_page_pool *p) {
     if (p == NULL || p->parts == NULL || p->refs == NULL || p->pages == NULL ||
         p->n_past == NULL || p->status == NULL)
@@ -95,6 +98,8 @@ int mynah_hip_pages_fork_dev(const mynah_page_pool *p, const int32_t *from, void
     pool_args(p, from, workspace, &a);
     hipStream_t st = mynah_stream_or_default(d, stream);
     void *args[] = {&a};
+    if (p->n_seqs <= 1024 && (uint64_t)p->n_seqs * p->max_pages <= 1024u * PAGES_FORK)
+        return mynah_launch(d, MYNAH_K_PAGES_FORK, 1, 1, 1024, 0, st, args);
     if (mynah_launch(d, MYNAH_K_PAGES_FORK_TAKE, p->n_seqs, 1, 256, 0, st, args) != 0) return -1;
     return mynah_launch(d, MYNAH_K_PAGES_FORK_GIVE, p->n_seqs, 1, 256, 0, st, args);
 }

@@ -58,6 +58,42 @@ extern "C" __global__ void __launch_bounds__(256) mynah_pages_fork_give(PageArgs
     if (threadIdx.x == 0u) a.n_past[b] = row[a.max_pages];
 }
 
+// A small table's in one launch of one workgroup: entries stay in registers between
+// the reads and the writes. Grid 1, block 1024; n_seqs <= 1024, n_seqs * max_pages <=
+// 1024 PG_FORK (8 sequences of 13 entries 4 us a call where two launches took 7, 128 of
+// 50 5 where they took 5.4).
+#define PG_FORK 8u                  // (= PAGES_FORK in pages.c)
+extern "C" __global__ void __launch_bounds__(1024) mynah_pages_fork(PageArgs a) {
+    const uint32_t tid = threadIdx.x, n = a.n_seqs * a.max_pages;
+    int32_t p[PG_FORK], was[PG_FORK];
+    bool mine[PG_FORK];
+#pragma unroll
+    for (uint32_t k = 0; k < PG_FORK; k++) {
+        const uint32_t i = tid + 1024u * k, b = i / a.max_pages;
+        const int32_t f = i < n ? a.ask[b] : 0;
+        mine[k] = i < n && (uint32_t)f != b;
+        p[k] = was[k] = -1;
+        if (mine[k]) {
+            was[k] = a.pages[i];
+            if ((uint32_t)f < a.n_seqs) p[k] = a.pages[(size_t)f * a.max_pages + (i - b * a.max_pages)];
+        }
+    }
+    int32_t past = 0;
+    const int32_t f = tid < a.n_seqs ? a.ask[tid] : (int32_t)tid;
+    if ((uint32_t)f != tid && (uint32_t)f < a.n_seqs) past = a.n_past[f];
+#pragma unroll
+    for (uint32_t k = 0; k < PG_FORK; k++) {
+        if (!mine[k] || was[k] == p[k]) continue;
+        if (is_page(a, was[k])) atomicSub(a.refs + was[k], 1);
+        if (is_page(a, p[k])) atomicAdd(a.refs + p[k], 1);
+    }
+    __syncthreads();                               // all have read
+#pragma unroll
+    for (uint32_t k = 0; k < PG_FORK; k++)
+        if (mine[k]) a.pages[tid + 1024u * k] = p[k];
+    if ((uint32_t)f != tid && tid < a.n_seqs) a.n_past[tid] = past;
+}
+
 // ── cutting sequences ───────────────────────────────────────────────────────
 // Grid n_seqs, block 256.
 extern "C" __global__ void __launch_bounds__(256) mynah_pages_release(PageArgs a) {
@@ -128,12 +164,34 @@ MYNAH_DEV PageSpan page_span(const PageArgs &a, uint32_t b) {
     return s;
 }
 
+// The place of page p in a table of 2 PG_T places in the LDS (-1: free) that PG_T
+// pages at most are put into.
+MYNAH_DEV uint32_t page_place(int32_t *keys, int32_t p) {
+    uint32_t h = (uint32_t)p * 2654435761u >> 21;  // 11 bits
+    for (;; h = (h + 1u) & (2u * PG_T - 1u)) {
+        const int32_t was = atomicCAS(keys + h, -1, p);
+        if (was == -1 || was == p) return h;
+    }
+}
+
 // Grid 1, block PG_T. Entries are taken sequence by sequence, K apiece, the longest
-// span: i is entry i % K of sequence i / K.
+// span: i is entry i % K of sequence i / K. Bound by reads that need each other: up to
+// PG_T entries each thread has its own, and counts and lists are in the LDS (of ten reads and
+// writes one after the other, in memory, 11 us).
 extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_reserve(PageArgs a) {
     __shared__ uint32_t longest, too_long, copies;
+    __shared__ int32_t keys[2u * PG_T], counts[2u * PG_T], firsts[2u * PG_T], given_to[PG_T];
     const uint32_t tid = threadIdx.x;
+    uint32_t first_free = 0u;                      // of pages 4 tid ..
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++)
+        first_free |= 4u * tid + k < a.n_pages && a.refs[4u * tid + k] <= 0 ? 1u << k : 0u;
     if (tid == 0u) longest = too_long = copies = 0u;
+    for (uint32_t k = tid; k < 2u * PG_T; k += PG_T) {
+        keys[k] = -1;
+        counts[k] = 0;
+        firsts[k] = 0x7fffffff;
+    }
     __syncthreads();
     for (uint32_t b = tid; b < a.n_seqs; b += PG_T) {
         const PageSpan s = page_span(a, b);
@@ -152,6 +210,75 @@ extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_reserve(PageArgs 
         at = a.pages + (size_t)b * a.max_pages + j;
         return j < s.to;
     };
+    // Free pages p .. p + 3 of `free`, `at` of them before: to the list as far as wanted.
+    auto list = [&](uint32_t p, uint32_t free, uint32_t at, uint32_t wanted, int32_t *to) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++)
+            if (free >> k & 1u) {
+                if (at < wanted) to[at] = (int32_t)(p + k);
+                at++;
+            }
+    };
+    auto free_of = [&](uint32_t p) {
+        uint32_t free = 0u;
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++)
+            free |= p + k < a.n_pages && a.refs[p + k] <= 0 ? 1u << k : 0u;
+        return free;
+    };
+    // An entry's page is given: 2 in place of a shared one, 3 with its content.
+    auto give = [&](int32_t get, int32_t *at, int32_t old, int32_t p) {
+        *at = p;
+        a.refs[p] = 1;
+        if (get > 1) atomicSub(a.refs + old, 1);
+        if (get == 3) {
+            const uint32_t c = atomicAdd(&copies, 1u);
+            ((int32_t *)a.from)[c] = old;
+            ((int32_t *)a.to)[c] = p;
+        }
+    };
+    auto with_content = [&](const PageSpan &s, uint32_t b, const int32_t *at) {
+        return (uint64_t)(at - (a.pages + (size_t)b * a.max_pages)) << a.page_log2 < s.past ? 3 : 2;
+    };
+    auto tell = [&](uint32_t wanted, uint32_t found) {
+        if (tid == 0u) {
+            a.status[0] = found < wanted ? (int32_t)(wanted - found) : 0;
+            a.status[1] = (int32_t)too_long;
+        }
+        return found >= wanted && too_long == 0u;
+    };
+    if (n <= PG_T) {
+        uint32_t b = 0u;
+        PageSpan s;
+        int32_t *at = nullptr, p = -1, r = 0, get = 0;
+        uint32_t h = 0u;
+        const bool in = entry(tid, b, s, at);
+        if (in) p = *at;
+        const bool held = in && is_page(a, p);
+        if (held) r = a.refs[p];
+        if (held && r > 1) {
+            h = page_place(keys, p);
+            atomicAdd(counts + h, 1);
+            atomicMin(firsts + h, (int32_t)b);
+        }
+        __syncthreads();
+        if (in && !held) get = 1;
+        else if (held && r > 1 && !(counts[h] == r && firsts[h] == (int32_t)b))
+            get = with_content(s, b, at);
+        uint32_t wanted, all;
+        const uint32_t k = before_me(get ? 1u : 0u, wanted);
+        uint32_t found = 0u;
+        for (uint32_t p0 = 0; p0 < a.n_pages && found < wanted; p0 += 4u * PG_T) {
+            const uint32_t free = p0 ? free_of(p0 + 4u * tid) : first_free;
+            list(p0 + 4u * tid, free, found + before_me(__popc(free), all), wanted, given_to);
+            found += all;
+        }
+        __syncthreads();
+        if (tell(wanted, found) && get) give(get, at, p, given_to[k]);
+        __syncthreads();
+        if (tid == 0u) *a.moves = (int32_t)copies;
+        return;
+    }
     // How many ask for a page that is there, and who first.
     for (int step = 0; step < 2; step++) {
         for (uint64_t i = tid; i < n; i += PG_T) {
@@ -183,8 +310,7 @@ extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_reserve(PageArgs 
             } else {
                 const int32_t r = a.refs[p];
                 if (r > 1 && !(fresh_i32(a.cnt + p) == r && fresh_i32(a.first + p) == (int32_t)b))
-                    get = (uint64_t)(at - (a.pages + (size_t)b * a.max_pages)) << a.page_log2 <
-                                  s.past ? 3 : 2;
+                    get = with_content(s, b, at);
             }
             a.rows[i0 + tid] = get;
         }
@@ -195,26 +321,14 @@ extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_reserve(PageArgs 
     // The lowest free pages, as many as are wanted.
     uint32_t found = 0u;
     for (uint32_t p0 = 0; p0 < a.n_pages && found < wanted; p0 += 4u * PG_T) {
-        const uint32_t p = p0 + 4u * tid;
-        uint32_t free = 0u;
-#pragma unroll
-        for (uint32_t k = 0; k < 4u; k++)
-            free |= p + k < a.n_pages && a.refs[p + k] <= 0 ? 1u << k : 0u;
-        uint32_t all, at = found + before_me(__popc(free), all);
-#pragma unroll
-        for (uint32_t k = 0; k < 4u; k++)
-            if (free >> k & 1u) {
-                if (at < wanted) a.list[at] = (int32_t)(p + k);
-                at++;
-            }
+        const uint32_t free = p0 ? free_of(p0 + 4u * tid) : first_free;
+        uint32_t all;
+        const uint32_t at = found + before_me(__popc(free), all);
+        list(p0 + 4u * tid, free, at, wanted, a.list);
         found += all;
     }
     page_sync();
-    const bool fits = found >= wanted && too_long == 0u;
-    if (tid == 0u) {
-        a.status[0] = found < wanted ? (int32_t)(wanted - found) : 0;
-        a.status[1] = (int32_t)too_long;
-    }
+    const bool fits = tell(wanted, found);
     uint32_t given = 0u;
     for (uint64_t i0 = 0; fits && i0 < n; i0 += PG_T) {
         uint32_t b;
@@ -224,17 +338,7 @@ extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_reserve(PageArgs 
         uint32_t all;
         const uint32_t k = given + before_me(get ? 1u : 0u, all);
         given += all;
-        if (get) {
-            const int32_t p = fresh_i32(a.list + k), old = *at;
-            *at = p;
-            a.refs[p] = 1;
-            if (get > 1) atomicSub(a.refs + old, 1);
-            if (get == 3) {
-                const uint32_t c = atomicAdd(&copies, 1u);
-                ((int32_t *)a.from)[c] = old;
-                ((int32_t *)a.to)[c] = p;
-            }
-        }
+        if (get) give(get, at, *at, fresh_i32(a.list + k));
     }
     __syncthreads();
     if (tid == 0u) *a.moves = (int32_t)copies;

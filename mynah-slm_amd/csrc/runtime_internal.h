@@ -259,6 +259,7 @@ enum { MYNAH_Q4_0 = 2, MYNAH_Q8_0 = 8, MYNAH_Q4_K = 12, MYNAH_Q5_K = 13, MYNAH_Q
     X(MYNAH_K_KV8_WIDE_BF16_E4M3_128, "mynah_kv8_wide_bf16_e4m3_128") \
     X(MYNAH_K_KV8_WIDE_BF16_I8_256, "mynah_kv8_wide_bf16_i8_256") \
     X(MYNAH_K_KV8_WIDE_BF16_E4M3_256, "mynah_kv8_wide_bf16_e4m3_256") \
+    X(MYNAH_K_PAGES_FORK, "mynah_pages_fork") \
     X(MYNAH_K_PAGES_FORK_TAKE, "mynah_pages_fork_take") \
     X(MYNAH_K_PAGES_FORK_GIVE, "mynah_pages_fork_give") \
     X(MYNAH_K_PAGES_RESERVE, "mynah_pages_reserve") \
