@@ -169,7 +169,9 @@ class Kv8:
         for b, (past, _) in enumerate(self.lens):
             past, nodes = max(past, 0), min(int(self.nodes[b]), self.max_nodes)
             end = min(past + nodes, self.max_kv)
-            rows = self.cache_rows(b, end) if end > past else []
+            if end <= past:
+                continue
+            rows = self.cache_rows(b, end)
             for first in range(past // self.block * self.block, end, self.block):
                 lo, hi = max(first, past), min(first + self.block, end)
                 if rows[lo] < 0:

@@ -289,3 +289,25 @@ def test_offsets_past_32_bits(M):
     M.kv8_attention_dev(a, ws.ptr, n)
     M.sync()
     c.check(c.raw())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("nodes", [1, 6, 20])
+def test_long_sequences_beside_short_ones(M, t, nodes):
+    """More pieces than CUs: sequences are cut by their lengths, pieces of 16 turns."""
+    lens = [(20_011, nodes), (3, 1), (9000, nodes), (0, 0), (14_500, 2)]
+    c = Kv8(M, lens, 4, 1, 128, t, E4M3, 64, page=64, seed=11)
+    raw = c.attend()
+    assert M.kv8_attention_workspace(c.attn_args()) > 12 * 130 * 4 * 16
+    c.check(raw)
+    assert np.array_equal(raw, c.attend())
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_a_prompt_cut_into_pieces(M, t):
+    # 96 tokens of one sequence over a long context: few workgroups of rows, so its
+    # positions are cut too.
+    c = Kv8(M, [(6000, 96)], 8, 2, 128, t, I8, 32, page=32, seed=12)
+    c.check(c.attend())
+    c = Kv8(M, [(3000, 40), (100, 96), (0, 3)], 4, 1, 64, t, E4M3, 16, mask="tree", seed=13)
+    c.check(c.attend())
