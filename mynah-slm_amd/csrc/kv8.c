@@ -108,7 +108,12 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *p, void *stream) {
     a.format = (uint32_t)c->format;
     /* The most blocks that max_nodes positions in a row touch. */
     a.blocks = (p->max_nodes + c->block - 2) / c->block + 1;
-    a.units = (unsigned long long)p->n_seqs * a.blocks * 2 * a.n_kv;
+    a.units = (unsigned long long)p->n_seqs * a.blocks;
+    /* A search of the sequence costs a microsecond or two, empty workgroups more where
+     * they are many. */
+    const unsigned long long few = p->n_rows / c->block + 2ull * p->n_seqs;
+    a.ragged = a.units > 4 * few + 4096;
+    a.units = (a.ragged ? few : a.units) * 2 * a.n_kv;
     /* A wave a block where a call's few rows fill no workgroup. */
     const uint32_t most = p->max_nodes < c->block ? p->max_nodes : c->block;
     const uint32_t wide = most * c->head_dim > 512u ? 1u : 0u;

@@ -20,8 +20,35 @@ struct Kv8StoreArgs {
     size_t slot_stride, seq_slots;
     unsigned long long n_slots, units;
     uint32_t n_seqs, n_kv, n_rows, page_log2, max_pages, block_log2, blocks, max_nodes, max_kv;
-    uint32_t format;
+    uint32_t format, ragged;
 };
+
+// Units of a ragged batch: sequence b's blocks are numbered from (its first row) / block
+// + 2 b on, which leaves room for its rows / block + 2 of them, all that so many rows
+// touch. The sequence of unit u is the last that begins at or before it, found by 64 lanes
+// at a time. (Numbered by the longest sequence, a prompt of 8000 tokens beside 255
+// single ones has 32,000 blocks, of which 380 are there.)
+MYNAH_DEV uint32_t kv8_sequence(const Kv8StoreArgs &a, unsigned long long u, uint32_t &i) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const long long row0 = a.seq_start[0];
+    auto begins = [&](uint32_t b) {
+        const long long rows = (long long)a.seq_start[b] - row0;
+        return (unsigned long long)((rows > 0 ? rows : 0) >> a.block_log2) + 2u * b;
+    };
+    uint32_t from = 0u, n = a.n_seqs;              // among from .. from + n - 1
+    while (n > 1u) {
+        const uint32_t step = (n + 63u) / 64u, b = from + lane * step;
+        const bool low = lane * step < n && begins(b) <= u;
+        const uint32_t upto = (uint32_t)__builtin_popcountll(__ballot(low));
+        const uint32_t at = upto ? (upto - 1u) * step : 0u;        // lane 0's is 0 in any case
+        from += at;
+        n = n - at < step ? n - at : step;
+    }
+    from = __builtin_amdgcn_readfirstlane(from);
+    const unsigned long long b0 = begins(from);
+    i = u - b0 < a.blocks ? (uint32_t)(u - b0) : a.blocks;         // past its last: no block
+    return from;
+}
 
 MYNAH_DEV float kv8_scale(float amax, uint32_t format) {
     if (format == KV_I8) return amax / 127.0f;
@@ -74,7 +101,9 @@ MYNAH_DEV void kv8_store(const Kv8StoreArgs &a) {
     u /= a.n_kv;
     const uint32_t kv = (uint32_t)(u & 1u);
     u >>= 1;
-    const uint32_t i = (uint32_t)(u % a.blocks), b = (uint32_t)(u / a.blocks);
+    uint32_t i = a.ragged ? 0u : (uint32_t)(u % a.blocks);
+    const uint32_t b = a.ragged ? kv8_sequence(a, u, i) : (uint32_t)(u / a.blocks);
+    if (i >= a.blocks) return;                     // uniform
     const long long row0 = a.seq_start[b], n = a.seq_start[b + 1u] - row0;
     const uint32_t past = a.n_past[b] > 0 ? (uint32_t)a.n_past[b] : 0u;
     const uint32_t nodes = n <= 0 ? 0u : n < (long long)a.max_nodes ? (uint32_t)n : a.max_nodes;

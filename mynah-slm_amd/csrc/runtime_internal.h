@@ -483,7 +483,7 @@ typedef struct {
     size_t slot_stride, seq_slots;
     unsigned long long n_slots, units;
     uint32_t n_seqs, n_kv, n_rows, page_log2, max_pages, block_log2, blocks, max_nodes, max_kv;
-    uint32_t format;
+    uint32_t format, ragged;
 } mynah_kv8_store_args;
 typedef struct {
     mynah_tree_args t;

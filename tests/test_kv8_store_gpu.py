@@ -43,6 +43,19 @@ def test_lengths(M, t, f, lens, page):
 
 
 @pytest.mark.parametrize("f", FORMATS)
+@pytest.mark.parametrize("n,where", [(70, 0), (70, 69), (300, 150), (5000, 3000)])
+def test_a_prompt_among_single_tokens(M, f, n, where):
+    """So many sequences, one of them long, that blocks are numbered by rows."""
+    rng = np.random.default_rng(n)
+    lens = [(int(a), int(b)) for a, b in zip(rng.integers(0, 20, n), rng.integers(0, 3, n))]
+    lens[where] = (13, 2400 if n < 1000 else 300)
+    c = Kv8(M, lens, 2, 1, 64, E.BF16, f, 16, seed=n, max_kv=2413, page=16 if n < 100 else 0,
+            extra_rows=3) if n < 1000 else \
+        Kv8(M, lens, 2, 1, 64, E.BF16, f, 16, seed=n, extra_rows=3)
+    c.check_store(c.store())
+
+
+@pytest.mark.parametrize("f", FORMATS)
 def test_scales_that_grow(M, f):
     # Small committed values under large new ones, and the other way round.
     for size in (1e-3, 1.0, 4.0, 1e4, 1e30):
