@@ -67,7 +67,7 @@ typedef struct {
  * filled is finite. All other rows stay as they were (of a block that is not full
  * the rows behind the new ones, too).
  *   - n_past, seq_start and pages are read on the device, so a captured call
- *     follows them; max_nodes bounds a sequence's new tokens and max_kv its
+ *     follows them; seq_start rises; max_nodes bounds a sequence's new tokens and max_kv its
  *     positions: tokens past either are not stored; a negative n_past counts as 0;
  *     token rows outside [0, n_rows) are not stored;
  *   - the blocks written are distinct: no two sequences of a call write to the
@@ -99,14 +99,20 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  *   out[row][h] = sum_p softmax_p(scale q[row][h] . k[p][h / group]) v[p][h / group]
  * over the seen positions, group = n_heads / n_kv_heads; a row that sees nothing is
  * 0. Unseen positions have no effect, whatever their codes are. A scale that is
- * not positive and finite counts as 0. An e4m3 NaN among the keys or the committed values makes the
- * rows that see it NaN; among the nodes' values it counts as 0.
+ * not positive and finite counts as 0. An e4m3 NaN among the keys or the committed
+ * values makes the rows that see it NaN; among the nodes' values it counts as 0.
  * Probabilities below 2^-126 of a row's largest count as 0.
- * Codes are widened exactly and products of f32 and f16 queries keep all their
+ *
+ * Codes are widened exactly, and products of f32 and f16 queries keep all their
  * bits; scores, statistics and sums are held in 32 bits. Each probability times
- * its value's scale is rounded for the product with V: to 8 bits of bf16 queries, 16 of f16,
- * not at all of f32; the result once, to `type`. The sums' order depends on the sizes, max_*
- * values and lengths alone, so equal calls give equal bits.
+ * its value's scale is rounded for the product with V: to 8 bits of bf16 queries,
+ * 16 of f16, not at all of f32; the result once, to `type`. The sums' order depends
+ * on the sizes, max_* values and lengths alone, so equal calls give equal bits.
+ *
+ * A call is planned for max_nodes: kernels of more than 32 rows a key head (nodes
+ * times group) leave a long sequence of one token to one workgroup a head. Where
+ * prompts and single tokens come together, one call for each kind is faster
+ * (seq_start, n_past and pages from a sequence on).
  *   - n_past, seq_start, pages and mask are read on the device; max_nodes and
  *     max_kv, rows outside [0, n_rows) and of no sequence, and a negative n_past as
  *     for the tree attention;
@@ -192,8 +198,8 @@ int mynah_hip_pages_reserve_dev(const mynah_page_pool *p, const int32_t *n_new, 
 int mynah_hip_pages_release_dev(const mynah_page_pool *p, const int32_t *keep, void *stream);
 
 /* The n pages in use move into the pages 0 .. n - 1: each page from n on, in rising
- * order, to the lowest free one, content, counts and table alike; what lies in the pages from n on
- * is free. status[0] becomes n, status[1] the number of pages that moved. */
+ * order, to the lowest free one, content, counts and table alike; the pages from n on
+ * are free then. status[0] becomes n, status[1] the number of pages that moved. */
 int mynah_hip_pages_compact_dev(const mynah_page_pool *p, void *workspace,
                                 size_t workspace_bytes, void *stream);
 

@@ -125,20 +125,21 @@ int mynah_hip_sample(mynah_hip_sampler *s, float *logits, uint32_t *id);
  *                l = l > 0 ? l / repeat[r] : l * repeat[r]
  *                l = l - freq[r] * c
  *                l = l - presence[r]
- *              MYNAH_PENALTY_ONCE: once for the token; MYNAH_PENALTY_EACH: c times over, as
- *              the sampler above does for its window (the same bits); NULL arrays
+ *              MYNAH_PENALTY_ONCE: once for the token; MYNAH_PENALTY_EACH: c times over,
+ *              as the sampler above does for its window (the same bits); NULL arrays
  *              stand for 1, 0 and 0
- *   biases     l = l + bias[k] where bias_id[k] = i, bias_start[r] <= k < bias_start[r +
- *              1]; of several such k the last
- *   grammars   -inf unless bit i % 32 of allowed[m][i / 32] is set, m = mask_row[r] (NULL: r);
- *              a row with m outside [0, n_masks) has none
- * rounded to out_type once. Ids outside [0, vocab) count for nothing. All pointers are device
- * pointers and everything but the sizes is read there, so a captured call follows it; calls are
- * asynchronous on `stream`, allocate nothing. hist, bias_id and allowed may be NULL: no
- * such rule. Starts rise and are 64-bit counts. Types are ggml's ids F32 = 0, F16 = 1, BF16 = 30;
- * strides count elements; y may be x with the same type and stride, otherwise they do not
- * overlap. mask_words >= ceil(vocab / 32); vocab < 2^31; elements on their own
- * size. 0, or -1 with the reason in mynah_hip_last_error(). */
+ *   biases     l = l + bias[k] where bias_id[k] = i, bias_start[r] <= k <
+ *              bias_start[r + 1]; of several such k the last
+ *   grammars   -inf unless bit i % 32 of allowed[m][i / 32] is set, m = mask_row[r]
+ *              (NULL: r); a row with m outside [0, n_masks) has none
+ * rounded to out_type once. Ids outside [0, vocab) count for nothing. hist, bias_id and
+ * allowed may be NULL: no such rule. All pointers are device pointers and everything
+ * but the sizes is read there, so a captured call follows it; calls are asynchronous
+ * on `stream` and allocate nothing. Starts rise and are 64-bit counts. Types are ggml's
+ * ids F32 = 0, F16 = 1, BF16 = 30; strides count elements; y may be x with the same
+ * type and stride, otherwise they do not overlap. mask_words >= ceil(vocab / 32); vocab <
+ * 2^31; elements on their own size. 0, or -1 with the reason in
+ * mynah_hip_last_error(). */
 enum { MYNAH_PENALTY_ONCE = 0, MYNAH_PENALTY_EACH = 1 };
 typedef struct {
     int type, out_type;

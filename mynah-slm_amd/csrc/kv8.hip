@@ -90,8 +90,11 @@ MYNAH_DEV void kv8_values(uint32_t d, uint32_t format, float *x) {
 
 // One workgroup of W waves takes one block of positions of a sequence, one head, of
 // keys or of values, so that a block's scale has one owner and no result depends on
-// an order. New values stay in registers between the largest and the rounding, up to HOLD runs of
-// eight a thread; further ones are read twice. Grid: units, heads fastest; block 64 W.
+// an order. New values stay in registers between the largest and the rounding, up to
+// HOLD runs of eight a thread; further ones are read twice. What bounds it: memory for
+// a prompt (8190 bf16 tokens of 8 heads of 128 to e4m3, 50 MB, 13.7 us, 3.7 TB/s), for
+// single tokens the launch and its reads one after the other (3.0-3.9 us, 256 tokens of
+// as many sequences 4.5). Grid: units, heads fastest; block 64 W.
 template <class T, int HD, int W, int HOLD>
 MYNAH_DEV void kv8_store(const Kv8StoreArgs &a) {
     constexpr uint32_t LPR = HD / 8, RPS = 64 * W / LPR; // lanes of a row, rows a step
@@ -494,8 +497,15 @@ struct Kv8Walk {
 // A workgroup's W waves take chunks of CK keys in turn, for the same 16 NT queries,
 // straight from memory into registers: a chunk's keys are under way while the one
 // before is weighed, its values while its scores are made. The waves' results meet
-// at the end. Grid slots * n_kv * groups (of 16 NT query rows), block 64 W; the order
-// of workgroups as in tree_attn.
+// at the end. Four waves and two workgroups a CU, so that one's start and end stand
+// beside the other's stream (one of eight: 170 us for 134, below). What bounds it:
+// memory, as far as two waves a SIMD keep copies under way (widening an e4m3 chunk is
+// 430 vector instructions, of i8 690, a quarter of the time). Measured: 32 sequences of
+// up to 16,384 positions, one bf16 token each, 554 MB, 134 us, 4.1 TB/s; 8 f16 nodes
+// over 130,009 i8 positions (266 MB) 67-74 us, 3.6-4.0 TB/s; 256 tokens over up to
+// 2048 bf16 positions (537 MB) 132 us; one f32 token over 513 12.1 us in two launches.
+// Grid slots * n_kv * groups (of 16 NT query rows), block 64 W; the order of
+// workgroups as in tree_attn.
 template <class T, int F, int HD, int NT>
 MYNAH_DEV void kv8_attn(const Kv8Args &g) {
     using S = Kv8Shape<T, HD, NT>;
@@ -763,6 +773,13 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
 // chunk ahead of values, so that the products of the next chunk's scores stand beside
 // this one's exponentials. Two buffers of each, one barrier a chunk. Places in the LDS are 16-byte pieces, swapped so that
 // 16 lanes of an access meet no bank twice.
+//
+// What bounds it: vector instructions (0.63 of the issue slots: 32 exponentials, their
+// sums and roundings, 32 codes to widen a lane and chunk) beside the products (0.39 of
+// the matrix cores' time); the LDS is busy 0.34. 2048 bf16 tokens behind 6144 i8 positions,
+// 32 heads, 8 of keys: 289-325 us by box, 0.74-0.83 PFLOP/s, where a large product
+// reaches 1.28; 2048 tokens of a new prompt 89 us; f16 queries 433 us (their weights are two
+// numbers), f32 630 (queries and weights three).
 template <class T, int HD>
 struct Kv8Wide {
     using S = Kv8Shape<T, HD>;

@@ -6,6 +6,11 @@
 // a row reads all of it), and which bias is each one's: integer sums and maxima, so
 // that no result depends on an order.
 //
+// What bounds it: memory, then the lists' latency and the LDS. 192 rows of 151,936, bf16 to
+// f32, histories of 2049 to 4096 tokens, biases, grammars (178 MB) 60 us, 2.9 TB/s; with
+// inputs in the last-level cache 42 us, 37 of them without biases, 27 with no rule
+// at all. Half or twice the tokens a workgroup 57 and 56 us for 47 then.
+//
 // SPDX-License-Identifier: MIT
 #pragma once
 #include "common.hip.h"

@@ -177,7 +177,8 @@ MYNAH_DEV uint32_t page_place(int32_t *keys, int32_t p) {
 // Grid 1, block PG_T. Entries are taken sequence by sequence, K apiece, the longest
 // span: i is entry i % K of sequence i / K. Bound by reads that need each other: up to
 // PG_T entries each thread has its own, and counts and lists are in the LDS (of ten reads and
-// writes one after the other, in memory, 11 us).
+// writes one after the other, in memory, 11 us; now 6.6 of the 16 us in which 8 sequences
+// are forked and get a page each, three launches).
 extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_reserve(PageArgs a) {
     __shared__ uint32_t longest, too_long, copies;
     __shared__ int32_t keys[2u * PG_T], counts[2u * PG_T], firsts[2u * PG_T], given_to[PG_T];
@@ -382,6 +383,8 @@ extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_compact(PageArgs 
 }
 
 // ── content ─────────────────────────────────────────────────────────────────
+// What bounds it: memory (150 pages of 6 layers, 118 MB read and as many written, 53 us,
+// 4.4 TB/s where a copy of a GiB reaches 5.0; chunks of 8 KiB 54, of 32 KiB 80).
 // Grid (workgroups a part, n_parts + 1), block 256: of the pairs in a.from and a.to
 // (a.moves of them, or a.count without), chunks of 16 KiB of one part. The last row of
 // workgroups brings the table up to date where a.map is given (compaction): entries

@@ -4,11 +4,14 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import os
+import re
 
 import pytest
 
 import mynah_amd as M
 from test_attention_ops import P, error
+from test_code_object import ROOT
 
 CACHE = dict(format=0, n_kv_heads=2, head_dim=128, block=32, k=P, v=P, slot_stride=256, n_slots=128,
              k_scale=P, v_scale=P, seq_slots=0, pages=P, page_size=64, max_pages=2)
@@ -125,3 +128,16 @@ def test_pool_arguments_refused():
         assert lib.mynah_hip_pages_reserve_dev(a, P, ws, n, None) == -1
         assert lib.mynah_hip_pages_compact_dev(a, ws, n, None) == -1
     assert lib.mynah_hip_pages_workspace(None) == 0
+
+
+# ── sizes that a kernel and its host code both state ─────────────────────────
+
+@pytest.mark.parametrize("host,host_name,source,kernel", [
+    ("kv8.c", r"#define KV8_WAVES (\d+)u", "kv8.hip", r"struct Kv8Shape \{.*?int W = (\d+);"),
+    ("kv8.c", r"#define KV8_WIDE_WAVES (\d+)u", "kv8.hip", r"struct Kv8Wide \{.*?int W = (\d+);"),
+    ("pages.c", r"#define PAGES_FORK (\d+)u", "pages.hip", r"#define PG_FORK (\d+)u")])
+def test_sizes_stated_twice_agree(host, host_name, source, kernel):
+    def value(path, pattern):
+        with open(os.path.join(ROOT, "mynah-slm_amd", "csrc", path)) as f:
+            return re.search(pattern, f.read(), re.S).group(1)
+    assert value(host, host_name) == value(source, kernel)
