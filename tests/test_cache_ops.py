@@ -43,7 +43,7 @@ def refused_attn(cache={}, **change):
     return why
 
 
-@pytest.mark.parametrize("change", BAD_CACHE, ids=str)
+@pytest.mark.parametrize("change", BAD_CACHE)
 def test_cache_refused(change):
     assert refused_store(change) and refused_attn(change)
 
@@ -53,7 +53,7 @@ def test_cache_refused(change):
     {"n_seqs": 65537}, {"n_rows": 0}, {"n_rows": 1 << 31}, {"max_nodes": 0},
     {"max_nodes": (1 << 24) + 1}, {"max_kv": 0}, {"max_kv": (1 << 26) + 1}, {"max_kv": 129},
     {"k_stride": 255}, {"v_stride": 128}, {"k_stride": 260}, {"k_stride": 1 << 62}, {"k": P + 8},
-    {"v": P + 2}, {"n_past": P + 2}, {"seq_start": P + 1}], ids=str)
+    {"v": P + 2}, {"n_past": P + 2}, {"seq_start": P + 1}])
 def test_store_refused(change):
     assert refused_store(**change)
     assert M.lib.mynah_hip_kv8_store_dev(None, None) == -1
@@ -66,7 +66,7 @@ def test_store_refused(change):
     {"max_kv": 129}, {"mask_words": 0}, {"max_nodes": 33}, {"q_stride": 1000}, {"out_stride": 512},
     {"q": P + 8}, {"out": P + 2}, {"q_stride": 1028}, {"mask": P + 2}, {"scale": math.nan},
     {"scale": math.inf}, {"q_stride": 1 << 61}, {"n_rows": 1 << 30, "mask_words": 8,
-                                                 "q_stride": 1024}], ids=str)
+                                                 "q_stride": 1024}])
 def test_attention_refused(change):
     assert refused_attn(**change)
 
@@ -100,7 +100,7 @@ BIG = 1 << 30
     {"n_pages": 0}, {"n_pages": 1 << 28}, {"n_seqs": 0}, {"n_seqs": 65537}, {"max_pages": 0},
     {"max_pages": 1 << 27}, {"page_size": 0}, {"page_size": 24}, {"n_parts": 0}, {"n_parts": 65535},
     {"parts": None}, {"refs": None}, {"pages": None}, {"n_past": None}, {"status": None},
-    {"parts": P + 4}, {"refs": P + 2}, {"status": P + 1}], ids=str)
+    {"parts": P + 4}, {"refs": P + 2}, {"status": P + 1}])
 def test_pool_refused(change):
     a = C.byref(M.PagePool(**{**POOL, **change}))
     lib = M.lib

@@ -24,7 +24,7 @@ GOOD = dict(type=30, out_type=0, n_rows=3, vocab=1000, x=P, x_stride=1000, y=P +
     {"bias_start": None}, {"mask_words": 31}, {"mask_words": 0}, {"x": P + 1}, {"y": P + 2},
     {"hist": P + 2}, {"hist_start": P + 4}, {"repeat": P + 1}, {"freq": P + 2}, {"presence": P + 3},
     {"bias_id": P + 2}, {"bias": P + 1}, {"bias_start": P + 4}, {"allowed": P + 2},
-    {"mask_row": P + 2}], ids=str)
+    {"mask_row": P + 2}])
 def test_refused(change):
     a = M.Logits(**{**GOOD, **change})
     assert M.lib.mynah_hip_logits_dev(C.byref(a), None) == -1
