@@ -104,7 +104,7 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  * Probabilities below 2^-126 of a row's largest count as 0.
  *
  * Codes are widened exactly, and products of f32 and f16 queries keep all their
- * bits; scores, statistics and sums are held in 32 bits. Each probability times
+ * bits (of f32 queries below 2^-100 in size the upper ones); scores, statistics and sums are held in 32 bits. Each probability times
  * its value's scale is rounded for the product with V: to 8 bits of bf16 queries,
  * 16 of f16, not at all of f32; the result once, to `type`. The sums' order depends
  * on the sizes, max_* values and lengths alone, so equal calls give equal bits.
@@ -116,7 +116,8 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  *   - n_past, seq_start, pages and mask are read on the device; max_nodes and
  *     max_kv, rows outside [0, n_rows) and of no sequence, and a negative n_past as
  *     for the tree attention;
- *   - out overlaps none of the inputs; queries are finite;
+ *   - out overlaps none of the inputs; queries are finite, scores (scale q . k)
+ *     below 2^29 in size;
  *   - 1 <= n_heads / n_kv_heads <= 64; q, out and strides aligned to 16 bytes;
  *     n_seqs and n_heads <= 65536, max_nodes <= 65535, max_kv <= 2^26, and
  *     with a mask max_nodes <= 32 * mask_words and n_rows * mask_words < 2^32. */

@@ -311,3 +311,36 @@ def test_a_prompt_cut_into_pieces(M, t):
     c.check(c.attend())
     c = Kv8(M, [(3000, 40), (100, 96), (0, 3)], 4, 1, 64, t, E4M3, 16, mask="tree", seed=13)
     c.check(c.attend())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("f", FORMATS)
+@pytest.mark.parametrize("nodes", [2, 60])
+def test_small_queries(M, t, f, nodes):
+    # f16 subnormals, and sizes at which the parts of an f32 are still normal bf16 numbers
+    size = {E.F32: 2.0 ** -90, E.F16: 2.0 ** -16, E.BF16: 2.0 ** -90}[t]
+    c = Kv8(M, [(100, nodes)], 4, 2, 64, t, f, seed=15, scale=0.2 / size)
+    c.q = E.encode(E.decode(c.q, t) * size, t)
+    c.check(c.attend())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nodes", [2, 60])
+@pytest.mark.parametrize("size", [2.0 ** 20, -2.0 ** 20, 2.0 ** 28])
+def test_equal_scores_of_any_size(M, t, hd, nodes, size):
+    """Every position scores the same: the mean of the values that a row sees, whatever
+    the size."""
+    c = Kv8(M, [(48, nodes)], 2, 1, hd, t, I8, seed=16)
+    c.k[:] = 3
+    c.ks[:] = np.float32(1 / 3)
+    c.q = E.encode(np.ones((nodes, 2 * hd)), t)
+    c.scale = size / hd
+    got = E.decode(c.attend(), t)
+    v = c.v.view(np.int8).astype(np.float64) * np.repeat(c.vs, 16, 0)
+    half = {E.F32: 0.0, E.F16: 2.0 ** -16, E.BF16: 2.0 ** -8}[t]
+    for i in range(nodes):
+        n = 48 + i + 1
+        want, big = v[:n].mean(0), np.abs(v[:n]).mean(0)
+        tol = (half + 4 * n * E.U) * big + E.rounded(want, t)
+        assert (np.abs(got[i].reshape(2, hd) - want) <= tol).all(), i
