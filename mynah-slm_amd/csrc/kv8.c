@@ -108,23 +108,23 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *p, void *stream) {
     a.format = (uint32_t)c->format;
     /* The most blocks that max_nodes positions in a row touch. */
     a.blocks = (p->max_nodes + c->block - 2) / c->block + 1;
-    a.units = (unsigned long long)p->n_seqs * a.blocks;
+    const unsigned long long all = (unsigned long long)p->n_seqs * a.blocks;
     /* A search of the sequence costs a microsecond or two, empty workgroups more where
      * they are many. */
     const unsigned long long few = p->n_rows / c->block + 2ull * p->n_seqs;
-    a.ragged = a.units > 4 * few + 4096;
-    a.units = (a.ragged ? few : a.units) * 2 * a.n_kv;
+    a.ragged = all > 4 * few + 4096;
+    const unsigned long long units = (a.ragged ? few : all) * 2 * a.n_kv;
     /* A wave a block where a call's few rows fill no workgroup. */
     const uint32_t most = p->max_nodes < c->block ? p->max_nodes : c->block;
     const uint32_t wide = most * c->head_dim > 512u ? 1u : 0u;
-    if (a.units > MYNAH_MOST_WGS(wide ? 256 : 64))
+    if (units > MYNAH_MOST_WGS(wide ? 256 : 64))
         return refuse("kv8_store: too many blocks for one launch");
     mynah_device *d = mynah_dev();
     if (d == NULL) return -1;
     const int h = c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2;
     void *args[] = {&a};
     return mynah_launch(d, MYNAH_K_KV8_STORE + 6 * type_index(p->type) + 2 * h + (int)wide,
-                        (unsigned)a.units, 1, wide ? 256 : 64, 0,
+                        (unsigned)units, 1, wide ? 256 : 64, 0,
                         mynah_stream_or_default(d, stream), args);
 }
 

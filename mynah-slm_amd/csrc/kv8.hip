@@ -18,7 +18,7 @@ struct Kv8StoreArgs {
     float *s[2];
     const int32_t *seq_start, *n_past, *pages;
     size_t slot_stride, seq_slots;
-    unsigned long long n_slots, units;
+    unsigned long long n_slots;
     uint32_t n_seqs, n_kv, n_rows, page_log2, max_pages, block_log2, blocks, max_nodes, max_kv;
     uint32_t format, ragged;
 };
@@ -227,11 +227,6 @@ struct Kv8Args {
 
 typedef uint32_t kv8_v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t kv8_v2u __attribute__((ext_vector_type(2)));
-
-typedef __attribute__((address_space(4))) const float kv8_const_f32;
-MYNAH_DEV float scalar_f32(const float *p, size_t i) {
-    return ((kv8_const_f32 *)(uintptr_t)p)[i];
-}
 
 template <class V>
 MYNAH_DEV uint32_t as_u32(V v) {
@@ -790,6 +785,8 @@ struct Kv8Wide {
     static constexpr int KS = HD / 32;              // steps of a score's product
     static constexpr int LB = HD == 64 ? 8 : 16;    // bytes of a thread's keys
     static constexpr int PR = CK / 8;               // pieces of a dimension's keys
+    // Steps by which LDS reads lead their products; f16's second number a weight leaves
+    // registers for two.
     static constexpr int AHEAD = S::F16 && HD == 128 ? 2 : 3;
 };
 

@@ -481,7 +481,7 @@ typedef struct {
     float *s[2];
     const int32_t *seq_start, *n_past, *pages;
     size_t slot_stride, seq_slots;
-    unsigned long long n_slots, units;
+    unsigned long long n_slots;
     uint32_t n_seqs, n_kv, n_rows, page_log2, max_pages, block_log2, blocks, max_nodes, max_kv;
     uint32_t format, ragged;
 } mynah_kv8_store_args;
