@@ -783,19 +783,19 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
 // ── many rows ───────────────────────────────────────────────────────────────
 //
 // A prompt's rows: the workgroup's waves share a chunk of CK keys, each with 16 NT
-// rows of its own. Every code is widened once a workgroup: a chunk's codes come into registers
-// while one before is computed, and leave for the LDS as bf16 (keys of f16 calls f16),
-// the values turned so that a lane reads eight keys of one dimension. Keys are a
-// chunk ahead of values, so that the products of the next chunk's scores stand beside
-// this one's exponentials. Two buffers of each, one barrier a chunk. Places in the LDS are 16-byte pieces, swapped so that
-// 16 lanes of an access meet no bank twice.
+// rows of its own. Every code is widened once a workgroup: a chunk's codes come into
+// registers while one before is computed, and leave for the LDS as bf16 (keys of f16
+// calls f16), the values turned so that a lane reads eight keys of one dimension. Keys
+// are a chunk ahead of values, so that the products of the next chunk's scores stand
+// beside this one's exponentials. Two buffers of each, one barrier a chunk. Places in
+// the LDS are 16-byte pieces, swapped so that 16 lanes of an access meet no bank twice.
 //
 // What bounds it: vector instructions (0.63 of the issue slots: 32 exponentials, their
 // sums and roundings, 32 codes to widen a lane and chunk) beside the products (0.39 of
 // the matrix cores' time); the LDS is busy 0.34. 2048 bf16 tokens behind 6144 i8 positions,
 // 32 heads, 8 of keys: 289-325 us by box, 0.74-0.83 PFLOP/s, where a large product
-// reaches 1.28; 2048 tokens of a new prompt 89 us; f16 queries 433 us (their weights are two
-// numbers), f32 630 (queries and weights three).
+// reaches 1.28; 2048 tokens of a new prompt 86 us; f16 queries 385 us (their weights are two
+// numbers), f32 584 (queries and weights three), on a box where bf16 takes 289.
 template <class T, int HD>
 struct Kv8Wide {
     using S = Kv8Shape<T, HD>;
