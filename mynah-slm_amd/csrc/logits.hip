@@ -7,9 +7,9 @@
 // that no result depends on an order.
 //
 // What bounds it: memory, then the lists' latency and the LDS. 192 rows of 151,936, bf16 to
-// f32, histories of 2049 to 4096 tokens, biases, grammars (178 MB) 60 us, 2.9 TB/s; with
-// inputs in the last-level cache 42 us, 37 of them without biases, 27 with no rule
-// at all. Half or twice the tokens a workgroup 57 and 56 us for 47 then.
+// f32, histories of 2049 to 4096 tokens, biases, grammars (178 MB) 60 us, 3.0 TB/s; with
+// inputs in the last-level cache 41 us, 38 of them without biases, 27 with no rule
+// at all. Half or twice the tokens a workgroup took 57 and 56 us for 47 in an earlier form.
 //
 // SPDX-License-Identifier: MIT
 #pragma once
@@ -97,9 +97,8 @@ template <class T, class O>
 MYNAH_DEV void logits(const LogitsArgs &a) {
 #pragma clang fp contract(off)
     constexpr uint32_t N = LG_CH / (4u * LG_T);    // runs of four tokens of a thread
-    // How often a token occurs, then which bias it gets, and whether one, a bit each.
+    // How often a token occurs; then, counted from 1, which bias it gets.
     __shared__ __attribute__((aligned(16))) uint32_t info[LG_CH];
-    __shared__ uint32_t moved[LG_CH / 32u];
     const uint32_t r = blockIdx.x / a.chunks, c0 = (blockIdx.x - r * a.chunks) * LG_CH;
     const uint32_t n = a.vocab - c0 < LG_CH ? a.vocab - c0 : LG_CH, tid = threadIdx.x;
     // The row's own first, then what depends on them and the logits, all at once: of
@@ -144,12 +143,11 @@ MYNAH_DEV void logits(const LogitsArgs &a) {
         const uint32_t i = 4u * (tid + LG_T * k);
         words[k] = masked && i < n ? allowed[i / 32u] : ~0u;
     }
-    if (count)
+    if (count || bias) {
 #pragma unroll
         for (uint32_t k = 0; k < N; k++) *(uint4 *)&info[4u * (tid + LG_T * k)] = uint4{0u, 0u, 0u, 0u};
-    if (bias)
-        for (uint32_t i = tid; i < LG_CH / 32u; i += LG_T) moved[i] = 0u;
-    if (count || bias) __syncthreads();
+        __syncthreads();
+    }
     if (count) {
         seen.each([&](uint32_t t, uint32_t) { atomicAdd(&info[t], 1u); });
         __syncthreads();
@@ -164,29 +162,27 @@ MYNAH_DEV void logits(const LogitsArgs &a) {
         for (uint32_t k = 0; k < N; k++) {
             const uint4 c4 = *(const uint4 *)&info[4u * (tid + LG_T * k)];
             const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
-            if (c4.x | c4.y | c4.z | c4.w)
+            if (c4.x | c4.y | c4.z | c4.w) {
+                if (bias) *(uint4 *)&info[4u * (tid + LG_T * k)] = uint4{0u, 0u, 0u, 0u};
 #pragma unroll
                 for (uint32_t j = 0; j < 4u; j++)
                     if (c[j]) v[k][j] = penalised(v[k][j], c[j], rep, freq, pres, a.each);
+            }
         }
     }
     if (bias) {
         if (count) __syncthreads();
-        wanted.each([&](uint32_t t, uint32_t) {
-            info[t] = 0u;
-            atomicOr(&moved[t / 32u], 1u << (t % 32u));
-        });
-        __syncthreads();
         // A bias by its place in the row's list; of several the last.
-        wanted.each([&](uint32_t t, uint32_t k) { atomicMax(&info[t], k); });
+        wanted.each([&](uint32_t t, uint32_t k) { atomicMax(&info[t], k + 1u); });
         __syncthreads();
 #pragma unroll
         for (uint32_t k = 0; k < N; k++) {
-            const uint32_t i = 4u * (tid + LG_T * k), c = moved[i / 32u] >> (i % 32u) & 15u;
-            if (c)
+            const uint4 w4 = *(const uint4 *)&info[4u * (tid + LG_T * k)];
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            if (w4.x | w4.y | w4.z | w4.w)
 #pragma unroll
                 for (uint32_t j = 0; j < 4u; j++)
-                    if (c >> j & 1u) v[k][j] += a.bias[b0 + info[i + j]];
+                    if (w[j]) v[k][j] += a.bias[b0 + (w[j] - 1u)];
         }
     }
 #pragma unroll
