@@ -136,9 +136,10 @@ int mynah_hip_sample(mynah_hip_sampler *s, float *logits, uint32_t *id);
  * allowed may be NULL: no such rule. All pointers are device pointers and everything
  * but the sizes is read there, so a captured call follows it; calls are asynchronous
  * on `stream` and allocate nothing. Starts rise and are 64-bit counts, each row's own
- * lists shorter than 2^32 - 1. Types are ggml's ids F32 = 0, F16 = 1, BF16 = 30; strides count elements; y may be x with the same
- * type and stride, otherwise they do not overlap. mask_words >= ceil(vocab / 32); vocab <
- * 2^31; elements on their own size. 0, or -1 with the reason in
+ * lists shorter than 2^32 - 1. Types are ggml's ids F32 = 0, F16 = 1, BF16 = 30;
+ * strides count elements; y may be x with the same type and stride, otherwise they do
+ * not overlap. mask_words >= ceil(vocab / 32); vocab < 2^31; elements on their own
+ * size. 0, or -1 with the reason in
  * mynah_hip_last_error(). */
 enum { MYNAH_PENALTY_ONCE = 0, MYNAH_PENALTY_EACH = 1 };
 typedef struct {
