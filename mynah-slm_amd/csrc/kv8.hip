@@ -117,6 +117,9 @@ MYNAH_DEV void kv8_store(const Kv8StoreArgs &a) {
     if (first64 >= end || past >= end) return;
     const uint32_t first = (uint32_t)first64, from = first < past ? past : first;
     const uint32_t upto = end - first < bs ? end : first + bs;
+    // A block none of whose rows are there keeps its scale.
+    const long long r0 = row0 + (long long)(from - past);
+    if (r0 >= (long long)a.n_rows || r0 + (long long)(upto - from) <= 0) return;
     unsigned long long slot = (unsigned long long)b * a.seq_slots + first;
     if (a.pages) {
         const int pg = a.pages[(size_t)b * a.max_pages + (first >> a.page_log2)];
