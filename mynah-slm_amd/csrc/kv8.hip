@@ -23,30 +23,30 @@ struct Kv8StoreArgs {
     uint32_t format, ragged;
 };
 
-// Units of a ragged batch: sequence b's blocks are numbered from (its first row) / block
-// + 2 b on, which leaves room for its rows / block + 2 of them, all that so many rows
-// touch. The sequence of unit u is the last that begins at or before it, found by 64 lanes
+// Units of a ragged batch: sequence b's blocks are numbered from (rows there before its
+// own) / block + 2 b on, which leaves room for its rows / block + 2 of them, all that so many
+// rows touch; a row is there in [0, n_rows), and a sequence's first block is its first such
+// row's. The sequence of unit u is the last that begins at or before it, found by 64 lanes
 // at a time. (Numbered by the longest sequence, a prompt of 8000 tokens beside 255
 // single ones has 32,000 blocks, of which 380 are there.)
 MYNAH_DEV uint32_t kv8_sequence(const Kv8StoreArgs &a, unsigned long long u, uint32_t &i) {
     const uint32_t lane = threadIdx.x & 63u;
-    const long long row0 = a.seq_start[0];
     auto begins = [&](uint32_t b) {
-        const long long rows = (long long)a.seq_start[b] - row0;
-        return (unsigned long long)((rows > 0 ? rows : 0) >> a.block_log2) + 2u * b;
+        const int32_t row = a.seq_start[b], there = row < (int32_t)a.n_rows ? row : (int32_t)a.n_rows;
+        return (unsigned long long)((uint32_t)(there > 0 ? there : 0) >> a.block_log2) + 2u * b;
     };
     uint32_t from = 0u, n = a.n_seqs;              // among from .. from + n - 1
     while (n > 1u) {
         const uint32_t step = (n + 63u) / 64u, b = from + lane * step;
         const bool low = lane * step < n && begins(b) <= u;
         const uint32_t upto = (uint32_t)__builtin_popcountll(__ballot(low));
-        const uint32_t at = upto ? (upto - 1u) * step : 0u;        // lane 0's is 0 in any case
+        const uint32_t at = upto ? (upto - 1u) * step : 0u;        // none: before the first's
         from += at;
         n = n - at < step ? n - at : step;
     }
     from = __builtin_amdgcn_readfirstlane(from);
     const unsigned long long b0 = begins(from);
-    i = u - b0 < a.blocks ? (uint32_t)(u - b0) : a.blocks;         // past its last: no block
+    i = u - b0 < a.blocks ? (uint32_t)(u - b0) : a.blocks;         // before or past its own: no block
     return from;
 }
 
@@ -113,7 +113,10 @@ MYNAH_DEV void kv8_store(const Kv8StoreArgs &a) {
     const unsigned long long all = (unsigned long long)past + nodes;
     const uint32_t end = all < a.max_kv ? (uint32_t)all : a.max_kv;
     const uint32_t bs = 1u << a.block_log2;
-    const unsigned long long first64 = (((unsigned long long)past >> a.block_log2) + i) << a.block_log2;
+    // Rows before row 0, whose blocks a ragged batch does not number.
+    const uint32_t skip = a.ragged && row0 < 0 ? (-row0 < (long long)nodes ? (uint32_t)-row0 : nodes) : 0u;
+    const unsigned long long first64 =
+        ((((unsigned long long)past + skip) >> a.block_log2) + i) << a.block_log2;
     if (first64 >= end || past >= end) return;
     const uint32_t first = (uint32_t)first64, from = first < past ? past : first;
     const uint32_t upto = end - first < bs ? end : first + bs;

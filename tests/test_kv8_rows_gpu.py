@@ -69,3 +69,19 @@ def test_blocks_that_get_no_row(M, f, hd):
     blocks = c.cache_rows(0, 80)[::16] // 16
     c.ks[blocks[1]], c.vs[blocks[2]], c.ks[blocks[0]] = np.nan, -1, 0
     c.check_store(c.store())
+
+
+@pytest.mark.parametrize("f", [I8, E4M3])
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("where", [0, 69])
+@pytest.mark.parametrize("shift,cut", [(-2300, 0), (-2420, 0), (-20, 0), (37, 0), (0, 50), (-2300, 30)])
+def test_ragged_batches_past_the_rows(M, f, page, where, shift, cut):
+    """One long sequence among many, so that blocks are numbered by rows, some of which
+    are before the first or behind the last one."""
+    rng = np.random.default_rng(1)
+    lens = [(int(a), int(b)) for a, b in zip(rng.integers(0, 20, 70), rng.integers(0, 4, 70))]
+    lens[where] = (13, 2400)
+    c = Rows(M, lens, 2, 1, 64, E.BF16, f, 16, page=page, seed=6)
+    c.move(shift, max(1, int(c.start[-1]) + shift - cut))
+    got = c.store()
+    c.check_store(got, (shift, cut))
