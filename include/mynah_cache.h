@@ -71,7 +71,8 @@ typedef struct {
  *     positions: tokens past either are not stored; a negative n_past counts as 0;
  *     token rows outside [0, n_rows) are not stored;
  *   - the blocks written are distinct: no two sequences of a call write to the
- *     same page (mynah_hip_pages_reserve_dev sees to that);
+ *     same page (mynah_hip_pages_reserve_dev sees to that), and without pages more
+ *     than one sequence with max_kv above seq_slots is refused;
  *   - k, v and their strides aligned to 16 bytes; the cache overlaps neither;
  *     n_seqs <= 65536, max_nodes <= 2^24, max_kv <= 2^26. */
 typedef struct {
@@ -117,6 +118,8 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  *   - n_past, seq_start, pages and mask are read on the device; max_nodes and
  *     max_kv, rows outside [0, n_rows) and of no sequence, and a negative n_past as
  *     for the tree attention;
+ *   - sequences may share cache rows (pages of one prefix, or without pages seq_slots
+ *     below max_kv, 0 for all the same rows);
  *   - out overlaps none of the inputs; queries are finite, scores (scale q . k)
  *     below 2^29 in size;
  *   - 1 <= n_heads / n_kv_heads <= 64; q, out and strides aligned to 16 bytes;

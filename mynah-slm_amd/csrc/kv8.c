@@ -74,6 +74,9 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *p, void *stream) {
         return refuse("kv8_store: bad counts (sequences, rows, tokens or positions)");
     const mynah_kv8_cache *c = &p->cache;
     if (cache_check(c, p->n_seqs, p->max_kv, "kv8_store") != 0) return -1;
+    /* Two sequences' rows may not meet: a block has one owner. */
+    if (c->pages == NULL && p->n_seqs > 1 && p->max_kv > c->seq_slots)
+        return refuse("kv8_store: max_kv positions do not fit seq_slots");
     const size_t row = (size_t)c->n_kv_heads * c->head_dim;
     if (p->k_stride < row || p->v_stride < row || !fits(p->n_rows, p->k_stride, row, size) ||
         !fits(p->n_rows, p->v_stride, row, size))
