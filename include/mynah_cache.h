@@ -102,7 +102,8 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  * 0. Unseen positions have no effect, whatever their codes are. A scale that is
  * not positive and finite counts as 0. An e4m3 NaN among the keys or the committed
  * values makes the rows that see it NaN; among the nodes' values it counts as 0.
- * Probabilities below 2^-126 of a row's largest count as 0.
+ * Probabilities below 2^-126 of a row's largest count as 0, and so does what of a
+ * weight (probability times value's scale) is below 2^-126.
  *
  * Codes are widened exactly, and products of f32 and f16 queries keep all their
  * bits (of f32 queries below 2^-100 in size the upper ones); scores, statistics and
@@ -120,8 +121,10 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  *     for the tree attention;
  *   - sequences may share cache rows (pages of one prefix, or without pages seq_slots
  *     below max_kv, 0 for all the same rows);
- *   - out overlaps none of the inputs; queries are finite, scores (scale q . k)
- *     below 2^29 in size;
+ *   - out overlaps none of the inputs; queries are below 2^110 in size (their products
+ *     with codes are summed before any scale), scores (scale q . k) below 2^29, values
+ *     (code times scale) below 2^93: up to 2^26 positions' probabilities, up to 2^8
+ *     before they are divided by their sum, meet in 32 bits;
  *   - 1 <= n_heads / n_kv_heads <= 64; q, out and strides aligned to 16 bytes;
  *     n_seqs and n_heads <= 65536, max_nodes <= 65535, max_kv <= 2^26, and
  *     with a mask max_nodes <= 32 * mask_words and n_rows * mask_words < 2^32. */

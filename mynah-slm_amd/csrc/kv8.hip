@@ -496,10 +496,12 @@ struct Kv8Walk {
         v = g.vs[i];
     }
     // As the products take them: the keys' times the call's, in log2 units; 0 unless
-    // positive and finite (the keys' next to it, so that -inf stays what it is).
+    // positive and finite. The keys' is f32's least number in place of 0, so that -inf
+    // stays what it is: 2^-149 of sums below 2^127 is 2^-22 of a score in log2 units.
+    // Below f32's normal numbers a factor is off by half of that, as much again.
     __device__ __forceinline__ void settle(float k, float v, float (&ks)[TILES],
                                            float (&vs)[TILES]) const {
-        k = fminf(fmaxf((k < INFINITY ? k : 0.0f) * g.scale2, 1e-30f), 3.402823466e38f);
+        k = fminf(fmaxf((k < INFINITY ? k : 0.0f) * g.scale2, 0x1p-149f), 3.402823466e38f);
         v = v > 0.0f && v < INFINITY ? v : 0.0f;
 #pragma unroll
         for (int t = 0; t < TILES; t++) {
