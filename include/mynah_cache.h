@@ -108,9 +108,10 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  * Codes are widened exactly, and products of f32 and f16 queries keep all their
  * bits (of f32 queries below 2^-100 in size the upper ones); scores, statistics and
  * sums are held in 32 bits. Each probability times its value's scale is rounded for
- * the product with V: to 8 bits of bf16 queries, 16 of f16, not at all of f32; the
- * result once, to `type`. The sums' order depends on the sizes, max_* values and
- * lengths alone, so equal calls give equal bits.
+ * the product with V: of f32 queries not at all, of f16 to 16 bits, of bf16 to 16 where
+ * max_nodes times group is 32 at most, to 8 from there on; the result once, to `type`.
+ * The sums' order depends on the sizes, max_* values and lengths alone, so equal calls
+ * give equal bits.
  *
  * A call is planned for max_nodes: kernels of more than 32 rows a key head (nodes
  * times group) leave a long sequence of one token to one workgroup a head. Where

@@ -220,9 +220,13 @@ KV8_STORES(bf16, __bf16)
 // the 16-bit type of the product: keys to bf16, or to f16 for f16 queries; values to
 // bf16, whose range holds a probability times any scale. What 16 bits do not hold
 // of the other operand goes into further products: f32 queries and weights are
-// three bf16 numbers each, weights of f16 calls two. The scales of a tile of 16 keys
-// are one number each: the keys' joins the exponent's factor (one fma a score),
-// the values' multiplies the probabilities.
+// three bf16 numbers each, weights of f16 calls two, and of bf16 calls two where rows are
+// few: memory bounds those (32 queries over up to 16,384 positions 134 us both ways, 256
+// over up to 2048 134 for 132). With many rows a bf16 call's weight is one number, 8 bits as
+// its result has: a second one takes 399 us for 292 of a prompt of 2048 behind 6144, and
+// halves the square of the error, which is the weights' and the result's rounding alike.
+// The scales of a tile of 16 keys are one number each: the keys' joins the exponent's
+// factor (one fma a score), the values' multiplies the probabilities.
 
 struct Kv8Args {
     TreeArgs t;                     // k and v codes; scale2 1, for the join of log2 references
@@ -291,7 +295,7 @@ template <class T, int HD, int NT = 1>
 struct Kv8Shape {
     static constexpr bool F32 = sizeof(T) == 4, F16 = __is_same(T, _Float16);
     static constexpr int QN = F32 ? 3 : 1;              // numbers that a query value is
-    static constexpr int PN = F32 ? 3 : F16 ? 2 : 1;    // ... that a weight is
+    static constexpr int PN = F32 ? 3 : 2;              // ... that a weight is
     static constexpr int TILES = HD * NT >= 256 ? 2 : 4; // 16-key tiles of a chunk
     static constexpr int CK = 16 * TILES;
     static constexpr int KP = HD / 64;                  // 16-byte pieces of a lane's key
@@ -528,8 +532,8 @@ struct Kv8Walk {
 // memory, as far as two waves a SIMD keep copies under way (widening an e4m3 chunk is
 // 430 vector instructions, of i8 690, a quarter of the time). Measured: 32 sequences of
 // up to 16,384 positions, one bf16 token each, 554 MB, 134 us, 4.1 TB/s; 8 f16 nodes
-// over 130,009 i8 positions (266 MB) 67-74 us, 3.6-4.0 TB/s; 256 tokens over up to
-// 2048 bf16 positions (537 MB) 132 us; one f32 token over 513 12.1 us in two launches.
+// over 130,009 i8 positions (266 MB) 67-74 us, 3.6-4.0 TB/s; 256 bf16 tokens over up to
+// 2048 i8 positions (537 MB) 134 us; one f32 token over 513 12.1 us in two launches.
 // Grid slots * n_kv * groups (of 16 NT query rows), block 64 W; the order of
 // workgroups as in tree_attn.
 template <class T, int F, int HD, int NT>
@@ -810,6 +814,7 @@ struct Kv8Wide {
     static constexpr int W = 8;
     static constexpr int NT = S::F32 || HD == 256 ? 1 : 2;  // column tiles of a wave
     static constexpr int ROWS = 16 * NT * W;
+    static constexpr int PN = S::F32 ? 3 : S::F16 ? 2 : 1;  // numbers that a weight is
     static constexpr int CK = HD == 256 ? 32 : 64, TILES = CK / 16;
     static constexpr int KS = HD / 32;              // steps of a score's product
     static constexpr int LB = HD == 64 ? 8 : 16;    // bytes of a thread's keys
@@ -1040,7 +1045,7 @@ MYNAH_DEV void kv8_wide(const Kv8Args &g) {
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) op[i] = key(1 - buf, i);
         kv8_refer(s[buf], ks, m, l, o);
-        uint32_t w[NT][TILES / 2][S::PN][4];
+        uint32_t w[NT][TILES / 2][Z::PN][4];
         constexpr int G = NT * TILES;              // tiles of all columns
 #pragma unroll
         for (int i = 0; i < SQ; i++) {
@@ -1061,7 +1066,7 @@ MYNAH_DEV void kv8_wide(const Kv8Args &g) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = S::PN - 1; j >= 0; j--)
+                for (int j = Z::PN - 1; j >= 0; j--)
                     o[n][i % S::VE] = ta_mfma<__bf16>(va, w[n][i / S::VE][j], o[n][i % S::VE]);
             if (i == SV / 4) widen_k(buf);
             if (i == SV / 2) widen_v(c + Z::CK, 1 - buf);

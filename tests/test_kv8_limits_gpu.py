@@ -1,12 +1,12 @@
 """Attention over an 8-bit cache at the ends of what it takes: factors of scores from
-f32's largest to below its smallest, and scales that count as 0 beside them."""
+f32's largest to below its smallest, scales that count as 0 beside them, weights' bits."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
 import elem_lib as E
-from kv8_lib import E4M3, I8, Kv8
+from kv8_lib import E4M3, I8, Kv8, values
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,29 @@ def test_scales_of_nothing_beside_large_queries(M, t, f, nodes, scale):
     c.ks[1], c.ks[3, 0], c.ks[3, 1], c.ks[5], c.ks[6] = 0, np.nan, np.inf, -1, 1e-45
     c.q = E.encode(E.decode(c.q, t) * LARGE[t], t)
     c.check(c.attend(), scale)
+
+
+@pytest.mark.parametrize("t", [E.F16, E.BF16])
+@pytest.mark.parametrize("f", FORMATS)
+@pytest.mark.parametrize("hd,nodes", [(64, 1), (64, 7), (128, 3), (128, 8), (256, 4)])
+def test_weights_of_few_rows(M, t, f, hd, nodes):
+    """Up to 32 rows a key head a weight keeps 16 bits: outputs are off by the result's
+    own rounding and 2^-16 of A = sum p |v|, besides what kv8_lib.Kv8.expected gives
+    scores, exponentials and sums (2 d A, 6 u A, and 2 n u A of two products a position)."""
+    past, heads, kvh = 57, 8, 2
+    c = Kv8(M, [(past, nodes)], heads, kvh, hd, t, f, 64, seed=hd + nodes)
+    got = E.decode(c.attend(), t)[:, :heads * hd].reshape(nodes, heads, hd)
+    k, v = ((values(x, f).reshape(-1, kvh, hd) * np.repeat(s.astype(np.float64), 64, 0)[..., None])
+            for x, s in ((c.k, c.ks), (c.v, c.vs)))
+    q = E.decode(c.q, t).reshape(nodes, heads, hd)
+    for i in range(nodes):
+        n = past + i + 1
+        for h in range(heads):
+            kk, vv = k[:n, h // 4], v[:n, h // 4]
+            x = c.scale * (kk @ q[i, h])
+            p = np.exp(x - x.max())
+            p /= p.sum()
+            d = (hd + 8) * E.U * c.scale * (np.abs(kk) @ np.abs(q[i, h])).max()
+            want, size = p @ vv, p @ np.abs(vv)
+            tol = (2 * d + (6 + 2 * n) * E.U + 2.0 ** -16) * size + E.rounded(want, t)
+            assert (np.abs(got[i, h] - want) <= tol).all(), (i, h)
