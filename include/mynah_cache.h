@@ -109,14 +109,20 @@ int mynah_hip_kv8_store_dev(const mynah_kv8_store *a, void *stream);
  * bits (of f32 queries below 2^-100 in size the upper ones); scores, statistics and
  * sums are held in 32 bits. Each probability times its value's scale is rounded for
  * the product with V: of f32 queries not at all, of f16 to 16 bits, of bf16 to 16 where
- * max_nodes times group is 32 at most, to 8 from there on; the result once, to `type`.
+ * max_nodes times group is 64 at most (32 with head_dim 256), to 8 from there on; the
+ * result once, to `type`.
  * The sums' order depends on the sizes, max_* values and lengths alone, so equal calls
  * give equal bits.
  *
- * A call is planned for max_nodes: kernels of more than 32 rows a key head (nodes
- * times group) leave a long sequence of one token to one workgroup a head. Where
- * prompts and single tokens come together, one call for each kind is faster
- * (seq_start, n_past and pages from a sequence on).
+ * A call is planned for max_nodes: kernels of many rows a key head (max_nodes times
+ * group above 64, or 32 where a query head is more than 256 bytes) leave a long sequence
+ * of one token to one workgroup a head. Where prompts and single tokens come together,
+ * one call for each kind is faster (seq_start, n_past and pages from a sequence on).
+ * Up to 255 sequences are cut by their lengths over the CUs while n_seqs times
+ * n_kv_heads times row groups is below the CUs' number, with few rows four times that;
+ * otherwise none is cut and the longest one sets the time: one of 130,000 positions beside
+ * 159 of 1000 1300 us (8 key heads, few rows), beside 100 of them 200. A call of
+ * its own for the long ones is faster.
  *   - n_past, seq_start, pages and mask are read on the device; max_nodes and
  *     max_kv, rows outside [0, n_rows) and of no sequence, and a negative n_past as
  *     for the tree attention;

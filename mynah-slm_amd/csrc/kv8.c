@@ -145,10 +145,14 @@ typedef struct {
 static void make_plan(const mynah_kv8_attention *p, uint32_t cus, kv8_plan *t) {
     const uint32_t group = p->n_heads / p->cache.n_kv_heads, hd = p->cache.head_dim;
     const uint64_t rows = (uint64_t)p->max_nodes * group;
-    /* From 33 rows on the shared chunk wins: four sequences of 16 nodes over 4000
-     * positions (bf16, 32 heads, 8 of keys, 64 rows a key head) 30 us for 38, of 32
-     * nodes over 8000 47 for 62; 96 rows of one sequence of 4000 24 both ways. */
-    t->wide = rows > 32;
+    /* Several workgroups of few rows read the same keys, each for itself; from some
+     * number of rows on the shared chunk wins. Few against wide in us, 32 heads, 8 of
+     * keys, i8, 4 sequences over 4000 positions, 64 rows a key head and 96: bf16 of 128
+     * values 28.2 and 30.2, 39.7 and 31.8; f16 28.0 and 35.5, 39.1 and 37.5; f32 of 64
+     * 23.1 and 25.0, 31.0 and 30.1. 32 sequences over 2000, 48 rows: 50 and 61 (bf16), 49
+     * and 80 (f16). Queries of more bytes lose earlier, 36 rows: bf16 of 256 45.7 and 36.2,
+     * f32 of 128 31.9 and 29.8. */
+    t->wide = rows > (hd * elem_size(p->type) <= 256 ? 64u : 32u);
     t->tiles = rows > 16 && hd != 256 ? 2u : 1u;
     t->waves = t->wide ? KV8_WIDE_WAVES : KV8_WAVES;
     t->rows = !t->wide ? 16u * t->tiles : p->type == MYNAH_F32 || hd == 256 ? 128u : 256u;

@@ -1,5 +1,6 @@
 """What either kernel of the attention over an 8-bit cache has of its own, few rows a
-key head (one and two column tiles, whole sequences and pieces) and many: e4m3's NaN,
+key head (one and two column tiles, one and two groups of rows, whole sequences and
+pieces) and many: e4m3's NaN,
 bad scales, offsets past 32 bits, cache rows that sequences share."""
 from __future__ import annotations
 
@@ -24,7 +25,7 @@ TYPES = [E.F32, E.F16, E.BF16]
 
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("hd", [64, 128, 256])
-@pytest.mark.parametrize("nodes", [5, 14, 40])
+@pytest.mark.parametrize("nodes", [5, 14, 25, 40])
 @pytest.mark.parametrize("past", [37, 5003])
 def test_nan(M, t, hd, nodes, past):
     """Behind the last position and in unseen nodes NaN reaches nobody; a seen node's

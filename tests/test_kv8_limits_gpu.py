@@ -60,9 +60,10 @@ def test_scales_of_nothing_beside_large_queries(M, t, f, nodes, scale):
 
 @pytest.mark.parametrize("t", [E.F16, E.BF16])
 @pytest.mark.parametrize("f", FORMATS)
-@pytest.mark.parametrize("hd,nodes", [(64, 1), (64, 7), (128, 3), (128, 8), (256, 4)])
+@pytest.mark.parametrize("hd,nodes", [(64, 1), (64, 7), (64, 16), (128, 3), (128, 8), (128, 13),
+                                      (256, 4), (256, 8)])
 def test_weights_of_few_rows(M, t, f, hd, nodes):
-    """Up to 32 rows a key head a weight keeps 16 bits: outputs are off by the result's
+    """Up to 64 rows a key head, 32 of 256 values, a weight keeps 16 bits: outputs are off by the result's
     own rounding and 2^-16 of A = sum p |v|, besides what kv8_lib.Kv8.expected gives
     scores, exponentials and sums (2 d A, 6 u A, and 2 n u A of two products a position)."""
     past, heads, kvh = 57, 8, 2
