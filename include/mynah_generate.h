@@ -125,6 +125,8 @@ int mynah_hip_sample(mynah_hip_sampler *s, float *logits, uint32_t *id);
  *                l = l > 0 ? l / repeat[r] : l * repeat[r]
  *                l = l - freq[r] * c
  *                l = l - presence[r]
+ *              one history for all three (where only some of them shall count a token,
+ *              two calls, the first to f32, the second in place there);
  *              MYNAH_PENALTY_ONCE: once for the token; MYNAH_PENALTY_EACH: c times over,
  *              as the sampler above does for its window (the same bits); NULL arrays
  *              stand for 1, 0 and 0

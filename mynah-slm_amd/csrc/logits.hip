@@ -7,9 +7,10 @@
 // that no result depends on an order.
 //
 // What bounds it: memory, then the lists' latency and the LDS. 192 rows of 151,936, bf16 to
-// f32, histories of 2049 to 4096 tokens, biases, grammars (178 MB) 60 us, 3.0 TB/s; with
-// inputs in the last-level cache 41 us, 38 of them without biases, 27 with no rule
-// at all. Half or twice the tokens a workgroup took 57 and 56 us for 47 in an earlier form.
+// f32, histories of 2049 to 4096 tokens, biases, grammars (178 MB) 60-65 us by box, 2.7-3.0
+// TB/s, 36 with no rule at all (4.9 TB/s), with the histories alone 60, biases 41, grammars
+// 38; with inputs in the last-level cache 41-44, and 27 with no rule. Half or twice the
+// tokens a workgroup took 57 and 56 us for 47 in an earlier form.
 //
 // SPDX-License-Identifier: MIT
 #pragma once

@@ -175,7 +175,8 @@ MYNAH_DEV uint32_t page_place(int32_t *keys, int32_t p) {
 }
 
 // Grid 1, block PG_T. Entries are taken sequence by sequence, K apiece, the longest
-// span: i is entry i % K of sequence i / K. Bound by reads that need each other: up to
+// span: i is entry i % K of sequence i / K, so that one long request among many short ones
+// costs as many rounds as if all were as long. Bound by reads that need each other: up to
 // PG_T entries each thread has its own, and counts and lists are in the LDS (of ten reads and
 // writes one after the other, in memory, 11 us; now 6.6 of the 16 us in which 8 sequences
 // are forked and get a page each, three launches).
@@ -298,7 +299,7 @@ extern "C" __global__ void __launch_bounds__(PG_T) mynah_pages_reserve(PageArgs 
         }
         page_sync();
     }
-    // Who gets a page: 1, with the content of its old one 2.
+    // Who gets a page: 1 where there is none, 2 in place of a shared one, 3 with its content.
     uint32_t wanted = 0u;
     for (uint64_t i0 = 0; i0 < n; i0 += PG_T) {
         uint32_t b;
