@@ -83,3 +83,14 @@ def test_weights_of_few_rows(M, t, f, hd, nodes):
             want, size = p @ vv, p @ np.abs(vv)
             tol = (2 * d + (6 + 2 * n) * E.U + 2.0 ** -16) * size + E.rounded(want, t)
             assert (np.abs(got[i, h] - want) <= tol).all(), (i, h)
+
+
+@pytest.mark.parametrize("t", [E.F32, E.BF16])
+@pytest.mark.parametrize("f", FORMATS)
+@pytest.mark.parametrize("past,nodes", [(100, 2), (5003, 12), (100, 60)])
+@pytest.mark.parametrize("size", [2.0 ** 90, 2.0 ** -100])
+def test_sizes_of_values(M, t, f, past, nodes, size):
+    """Values near the largest that are taken, and of the least scale that the store makes."""
+    c = Kv8(M, [(past, nodes)], 4, 2, 128, t, f, 64, seed=18, mask="tree")
+    c.vs = (c.vs * np.float32(size)).astype(np.float32)
+    c.check(c.attend(), size)
