@@ -205,8 +205,8 @@ int mynah_hip_pages_fork_dev(const mynah_page_pool *p, const int32_t *from, void
  * sequences and positions. n_past stays as it is. status[0] is the number of pages
  * that were missing, status[1] of sequences that would not fit max_pages entries: unless
  * both are 0, nothing has changed. The time grows with n_seqs times the most entries that
- * one sequence asks for: a page each for 256 sequences 5 us, with one of them asking for
- * 125 112 us, for 512 373. */
+ * one sequence asks for: room for a token for each of 256 sequences 5 us, with 125 pages
+ * for one of them 112 us, with 512 373. */
 int mynah_hip_pages_reserve_dev(const mynah_page_pool *p, const int32_t *n_new, void *workspace,
                                 size_t workspace_bytes, void *stream);
 

@@ -804,10 +804,13 @@ MYNAH_DEV void kv8_attn(const Kv8Args &g) {
 //
 // What bounds it: vector instructions (0.63 of the issue slots: 32 exponentials, their
 // sums and roundings, 32 codes to widen a lane and chunk) beside the products (0.39 of
-// the matrix cores' time); the LDS is busy 0.34. 2048 bf16 tokens behind 6144 i8 positions,
-// 32 heads, 8 of keys: 289-325 us by box, 0.74-0.83 PFLOP/s, where a large product
-// reaches 1.28; 2048 tokens of a new prompt 86 us; f16 queries 385 us (their weights are two
-// numbers), f32 584 (queries and weights three), on a box where bf16 takes 289.
+// the matrix cores' time); the LDS is busy 0.34. Then a chain's rows: a workgroup a CU
+// stops at the last position its rows see, and the last one's sets the time. 2048 bf16
+// tokens behind 6144 i8 positions, 32 heads, 8 of keys (7168 positions in the mean, 8192
+// for the last rows): 289-331 us by box, 0.73-0.83 PFLOP/s, where a large product reaches
+// 1.28; 2048 tokens of a new prompt (1 to 32 chunks) 86-92 us; f16 queries 385 us (their
+// weights are two numbers), f32 584 (queries and weights three), on a box where bf16
+// takes 289.
 template <class T, int HD>
 struct Kv8Wide {
     using S = Kv8Shape<T, HD>;
